@@ -1,0 +1,404 @@
+"""The attention half of a layer as measurable cases: rotary positions, a paged key-value cache in fp16 or e4m3, attention
+over packed prompts and of one new token over the cache.
+
+A case names the operator and its sizes.  Lengths of the sequences follow from the case alone (`_lengths`), values from
+the seed.  `run` computes the plain form; where the module's `own` is true it calls the library instead.
+"""
+import math
+
+import torch
+
+own = False
+
+# query heads, key-value heads, head size: the two named shapes' width of 2048, the small configurations, and odd groups
+HEADS = {"32x4x128": (32, 4, 128), "16x2x128": (16, 2, 128), "32x16x64": (32, 16, 64), "4x2x64": (4, 2, 64),
+         "16x16x128": (16, 16, 128), "12x4x64": (12, 4, 64), "14x2x128": (14, 2, 128), "16x1x64": (16, 1, 64)}
+THETA = 1e6
+MOST_PAIRS = 32 * 8192 * 8192     # heads x queries x keys of the largest padded prompt batch
+MOST_CACHED = 4 * 128 * 560000    # kv heads x head size x cached tokens of the largest decode batch
+
+
+def listed():
+    return [
+        # a decode step's projections before the cache and the attention
+        {"name": "rope-16", "op": "rope", "heads": "32x4x128", "rows": 16, "rot": 128},
+        # a prompt chunk of the larger batch, half of every head rotated, positions far into a long text
+        {"name": "rope-4096", "op": "rope", "heads": "32x4x128", "rows": 4096, "rot": 64},
+        # one new token of each of 129 sequences into a quantised cache
+        {"name": "write-129", "op": "write", "heads": "32x4x128", "rows": 129, "step": True, "page": 64, "type": "e4m3"},
+        # a prompt batch into a quantised cache
+        {"name": "write-16384", "op": "write", "heads": "16x16x128", "rows": 16384, "step": False, "page": 32, "type": "e4m3"},
+        # a cached prefix of a small model read back for the next chunk of its prompt, pages left half full
+        {"name": "read-1003", "op": "read", "heads": "4x2x64", "seqs": 3, "longest": 1003, "page": 16, "type": "fp16"},
+        # quantised prefixes of a batch of prompts
+        {"name": "read-8191", "op": "read", "heads": "32x4x128", "seqs": 12, "longest": 8191, "page": 64, "type": "e4m3"},
+        # the teacher's windows of 384 tokens, a batch of them packed
+        {"name": "attn-windows", "op": "attn", "heads": "16x2x128", "seqs": 32, "longest": 384, "past": 0, "ragged": False},
+        # packed prompts of different lengths behind cached prefixes, odd group
+        {"name": "attn-ragged", "op": "attn", "heads": "12x4x64", "seqs": 13, "longest": 1999, "past": 517, "ragged": True},
+        # one long prompt
+        {"name": "attn-8192", "op": "attn", "heads": "32x4x128", "seqs": 1, "longest": 8192, "past": 0, "ragged": False},
+        # one sequence's next token: latency
+        {"name": "decode-1", "op": "decode", "heads": "32x4x128", "seqs": 1, "longest": 777, "page": 64, "type": "fp16"},
+        # a small batch over long quantised caches
+        {"name": "decode-16", "op": "decode", "heads": "32x4x128", "seqs": 16, "longest": 16384, "page": 64, "type": "e4m3"},
+        # a large ragged batch
+        {"name": "decode-129", "op": "decode", "heads": "32x4x128", "seqs": 129, "longest": 8191, "page": 32, "type": "fp16"},
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number from lo to hi, evenly over its logarithm."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))
+
+
+def draw(rng):
+    op = rng.choice(["rope", "write", "read", "attn", "attn", "attn", "decode", "decode", "decode"])
+    heads = rng.choice(sorted(HEADS))
+    h, g, d = HEADS[heads]
+    case = {"op": op, "heads": heads}
+    if op == "rope":
+        return dict(case, rows=_spread(rng, 1, 4096), rot=rng.choice([d, d, d // 2, 48]))
+    if op == "attn":
+        seqs = _spread(rng, 1, 48)
+        top = min(8192, int(math.sqrt(MOST_PAIRS / (seqs * h))))
+        longest = _spread(rng, 1, top)
+        past = rng.choice([0, 0, rng.randint(1, 700)])
+        if longest * (longest + past) > top * top:
+            past = 0
+        return dict(case, seqs=seqs, longest=longest, past=past, ragged=rng.random() < 0.6)
+    case.update(page=rng.choice([16, 32, 64, 128]), type=rng.choice(["fp16", "e4m3"]))
+    if op == "write":
+        step = rng.random() < 0.5
+        return dict(case, rows=_spread(rng, 1, 512 if step else 16384 * 2048 // max(2048, g * d)), step=step)
+    seqs = _spread(rng, 1, 200 if op == "decode" else 24)
+    top = min(65536 if op == "decode" else 8191, MOST_CACHED // (g * d * seqs))
+    if op == "read":
+        top = min(top, 12 * 8191 * 512 // (g * d * seqs))
+    return dict(case, seqs=seqs, longest=_spread(rng, 1, top))
+
+
+def _lengths(seqs, longest, ragged=True):
+    """Lengths of a batch: all the longest, or spread evenly from one token to the longest in a mixed order."""
+    if not ragged:
+        return [longest] * seqs
+    return [longest if i == 0 else 1 + int((longest - 1) * ((i * 0.6180339887498949) % 1.0)) for i in range(seqs)]
+
+
+# ---- what a user's program has in hand ---------------------------------------------------------
+class _Make:
+    """Seeded tensors on the GPU."""
+
+    def __init__(self, seed):
+        self.gen = torch.Generator(device="cuda")
+        self.gen.manual_seed(int(seed))
+
+    def f32(self, *shape):
+        return torch.randn(shape, device="cuda", generator=self.gen)
+
+    def f16(self, *shape):
+        out = torch.empty(shape, device="cuda", dtype=torch.float16)
+        return out.normal_(generator=self.gen)
+
+    def order(self, n):
+        return torch.randperm(n, device="cuda", generator=self.gen).int()
+
+
+def _starts(lengths):
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+
+def _scales(x):
+    """Power-of-two scale of e4m3 codes (largest 448 = 0.875 * 2^9) for the last dimension."""
+    m, e = torch.frexp(x.float().abs().amax(-1))
+    return torch.where(m == 0, torch.ones_like(m), torch.ldexp(torch.ones_like(m), torch.where(m <= 0.875, e - 9, e - 8)))
+
+
+def _cache(mk, case, pages):
+    """A cache filled with what earlier steps have written."""
+    _, g, d = HEADS[case["heads"]]
+    kv = {"pages": pages}
+    for n in ("k", "v"):
+        x = mk.f16(pages, g, case["page"], d)
+        if case["type"] == "e4m3":
+            kv[n + "_scale"] = _scales(x)
+            for lo in range(0, pages, 1024):   # in pieces, so that the fp32 form is never whole
+                s = kv[n + "_scale"][lo:lo + 1024, ..., None]
+                x[lo:lo + 1024] = x[lo:lo + 1024] / s
+            x = x.to(torch.float8_e4m3fn)
+        kv[n] = x
+    return kv
+
+
+def prepare(case, seed):
+    mk = _Make(seed)
+    h, g, d = HEADS[case["heads"]]
+    op = case["op"]
+    s = {"case": case}
+    if op == "rope":
+        rows = case["rows"]
+        s["x"] = mk.f32(rows, (h + 2 * g) * d)
+        s["pos"] = torch.randint(0, 131072, (rows,), device="cuda", generator=mk.gen, dtype=torch.int32)
+        s["out"] = torch.empty(rows, (h + 2 * g) * d, device="cuda", dtype=torch.float16)
+        return s
+    if op == "write":
+        rows, page = case["rows"], case["page"]
+        # keys and values where the projection left them, behind the queries
+        s["p16"] = mk.f16(rows, (h + 2 * g) * d)
+        # pages in the order in which they came free: a row of each sequence somewhere in a page of its own, or whole pages in turn
+        used = rows if case["step"] else -(-rows // page)
+        s["kv"] = _cache(mk, case, used + 3)
+        order, row = mk.order(used + 3), torch.arange(rows, device="cuda")
+        place = torch.randint(0, page, (rows,), device="cuda", generator=mk.gen)
+        s["slot"] = (order[row] * page + place if case["step"] else order[row // page] * page + row % page).int()
+        return s
+    if op == "attn":
+        lq = _lengths(case["seqs"], case["longest"], case["ragged"])
+        lk = [n + case["past"] for n in lq]
+        s.update(cu_q=_starts(lq), cu_k=_starts(lk), lq=max(lq), lk=max(lk))
+        s["q"], s["k"], s["v"] = mk.f16(sum(lq), h, d), mk.f16(sum(lk), g, d), mk.f16(sum(lk), g, d)
+        s["out"] = torch.empty_like(s["q"])
+        return s
+    lengths, page = _lengths(case["seqs"], case["longest"]), case["page"]
+    per = -(-case["longest"] // page)
+    need = [-(-n // page) for n in lengths]
+    s["kv"] = _cache(mk, case, sum(need))
+    order, table, at = mk.order(sum(need)), torch.zeros(len(need), per, dtype=torch.int32, device="cuda"), 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n]
+        at += n
+    s["table"] = table
+    if op == "read":
+        s["cu"] = _starts(lengths)
+        s["rows"] = sum(lengths)
+        s["k"], s["v"] = (torch.empty(s["rows"], g, d, device="cuda", dtype=torch.float16) for _ in range(2))
+    else:
+        s["len"] = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        s["q"] = mk.f16(len(lengths), h, d)
+        s["out"] = torch.empty_like(s["q"])
+    return s
+
+
+# ---- one pass: the plain forms -----------------------------------------------------------------
+def _rope(s):
+    case = s["case"]
+    h, g, d = HEADS[case["heads"]]
+    half = case["rot"] // 2
+    x = s["x"].view(-1, h + 2 * g, d)
+    i = torch.arange(half, device=x.device, dtype=torch.float64)
+    a = s["pos"].double()[:, None] * torch.pow(torch.tensor(THETA, dtype=torch.float64, device=x.device), -i / half)
+    cos, sin = a.cos().float()[:, None], a.sin().float()[:, None]
+    y = x.clone()
+    lo, hi = x[:, :h + g, :half], x[:, :h + g, half:2 * half]
+    y[:, :h + g, :half] = lo * cos - hi * sin
+    y[:, :h + g, half:2 * half] = hi * cos + lo * sin
+    return y.view(s["x"].shape).half()
+
+
+def _write(s):
+    case, kv = s["case"], s["kv"]
+    h, g, d = HEADS[case["heads"]]
+    p = s["p16"].view(-1, h + 2 * g, d)
+    slot = s["slot"].long()
+    page, place = slot // case["page"], slot % case["page"]
+    for n, x in (("k", p[:, h:h + g]), ("v", p[:, h + g:])):
+        if case["type"] == "fp16":
+            kv[n][page, :, place] = x
+        else:
+            scale = _scales(x)
+            kv[n + "_scale"][page, :, place] = scale
+            kv[n].view(torch.uint8)[page, :, place] = (x.float() / scale[..., None]).to(torch.float8_e4m3fn).view(torch.uint8)
+    return [kv[n] for n in ("k", "v", "k_scale", "v_scale") if n in kv]
+
+
+def _gather(s, n, rows, seq, place):
+    """Cached rows of sequence and place as fp32."""
+    kv, page = s["kv"], s["case"]["page"]
+    at = s["table"].long()[seq, place // page]
+    x = kv[n].view(torch.uint8)[at, :, place % page].view(torch.float8_e4m3fn) if n + "_scale" in kv else kv[n][at, :, place % page]
+    x = x.float()
+    return x * kv[n + "_scale"][at, :, place % page][..., None] if n + "_scale" in kv else x
+
+
+def _read(s):
+    row = torch.arange(s["rows"], device="cuda")
+    cu = s["cu"].long()
+    seq = torch.searchsorted(cu, row, right=True) - 1
+    return [_gather(s, n, s["rows"], seq, row - cu[seq]).half() for n in ("k", "v")]
+
+
+def _softmax_product(q, k, v, seen, scale):
+    """q [n, i, g, m, d], k and v [n, j, g, d], seen [n, i, j]; a row that sees nothing gives zero."""
+    score = torch.einsum("nigmd,njgd->ngmij", q, k) * scale
+    score = score.masked_fill_(~seen[:, None, None], -math.inf)
+    top = score.amax(-1, keepdim=True)
+    p = score.sub_(torch.where(top == -math.inf, torch.zeros_like(top), top)).exp_()
+    total = p.sum(-1, keepdim=True)
+    o = torch.einsum("ngmij,njgd->ngmid", p, v) / torch.where(total == 0, torch.ones_like(total), total)
+    return o.permute(0, 3, 1, 2, 4).reshape(q.shape[0], q.shape[1], -1, q.shape[-1])
+
+
+def _attn(s):
+    h, g, d = HEADS[s["case"]["heads"]]
+    cq, ck = s["cu_q"].long(), s["cu_k"].long()
+    lq, lk = (cq[1:] - cq[:-1])[:, None], (ck[1:] - ck[:-1])[:, None]
+    i, j = torch.arange(s["lq"], device="cuda"), torch.arange(s["lk"], device="cuda")
+    at_q, at_k = (cq[:-1, None] + i).clamp_(max=s["q"].shape[0] - 1), (ck[:-1, None] + j).clamp_(max=s["k"].shape[0] - 1)
+    seen = j[None, None, :] <= i[None, :, None] + (lk - lq)[:, :, None]
+    seen &= (j < lk)[:, None, :]
+    o = _softmax_product(s["q"][at_q].float().view(*at_q.shape, g, h // g, d), s["k"][at_k].float(), s["v"][at_k].float(), seen, d ** -0.5)
+    return o[i < lq].half()
+
+
+def _decode(s):
+    h, g, d = HEADS[s["case"]["heads"]]
+    n = s["q"].shape[0]
+    j = torch.arange(s["case"]["longest"], device="cuda")
+    seq = torch.arange(n, device="cuda")[:, None].expand(n, j.numel())
+    k, v = (_gather(s, name, n, seq, j.expand_as(seq)) for name in ("k", "v"))
+    seen = (j < s["len"][:, None])[:, None]
+    v = v.masked_fill_(~seen[:, 0, :, None, None], 0.0)
+    return _softmax_product(s["q"].float().view(n, 1, g, h // g, d), k, v, seen, d ** -0.5).view(n, h, d).half()
+
+
+PLAIN = {"rope": _rope, "write": _write, "read": _read, "attn": _attn, "decode": _decode}
+
+
+# ---- one pass: the library's calls -------------------------------------------------------------
+_held = {}
+
+
+def _library():
+    """A program's one context, on a stream of its own."""
+    if not _held:
+        import __graft_entry__ as entry
+
+        mc = entry.load_package().moe_cuda
+        stream = torch.cuda.Stream()
+        _held.update(mc=mc, stream=stream, ctx=mc.Ctx(torch.cuda.current_device(), stream.cuda_stream))
+        _held["ctx"].check()
+    return _held["mc"], _held["ctx"]
+
+
+def _kv(mc, s):
+    kv, (_, g, d) = s["kv"], HEADS[s["case"]["heads"]]
+    at = {n: kv[n].data_ptr() if n in kv else None for n in ("k", "v", "k_scale", "v_scale")}
+    kind = mc.KV_E4M3 if s["case"]["type"] == "e4m3" else mc.KV_F16
+    return mc.Kv(pages=kv["pages"], page=s["case"]["page"], kv_heads=g, hd=d, type=kind, **at)
+
+
+def _call(s):
+    mc, ctx = _library()
+    case = s["case"]
+    h, g, d = HEADS[case["heads"]]
+    op = case["op"]
+    if op == "rope":
+        ctx.rope(s["x"].data_ptr(), s["pos"].data_ptr(), s["out"].data_ptr(), case["rows"], h + 2 * g, h + g, d, case["rot"], THETA)
+        out = s["out"]
+    elif op == "write":
+        at = s["p16"].data_ptr()
+        ctx.kv_write(_kv(mc, s), at + 2 * h * d, at + 2 * (h + g) * d, s["slot"].data_ptr(), case["rows"], (h + 2 * g) * d)
+        out = [s["kv"][n] for n in ("k", "v", "k_scale", "v_scale") if n in s["kv"]]
+    elif op == "read":
+        ctx.kv_read(_kv(mc, s), s["table"].data_ptr(), s["cu"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), case["seqs"],
+                    s["rows"], s["table"].shape[1])
+        out = [s["k"], s["v"]]
+    elif op == "attn":
+        ctx.attn(s["q"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), s["cu_q"].data_ptr(), s["cu_k"].data_ptr(), s["out"].data_ptr(),
+                 case["seqs"], s["q"].shape[0], s["k"].shape[0], h, g, d)
+        out = s["out"]
+    else:
+        ctx.attn_decode(_kv(mc, s), s["q"].data_ptr(), s["table"].data_ptr(), s["len"].data_ptr(), s["out"].data_ptr(), case["seqs"], h,
+                        case["longest"], s["table"].shape[1])
+        out = s["out"]
+    ctx.check()   # a refused call shows here; nothing is waited for
+    return out
+
+
+def run(state):
+    return _call(state) if own else PLAIN[state["case"]["op"]](state)
+
+
+# ---- what a pass cannot do without -------------------------------------------------------------
+def work(case):
+    h, g, d = HEADS[case["heads"]]
+    op = case["op"]
+    if op == "rope":
+        return {"bytes": case["rows"] * ((h + 2 * g) * d * 6 + 4), "flops": case["rows"] * (h + g) * case["rot"] * 3.0}
+    if op == "attn":
+        lq = _lengths(case["seqs"], case["longest"], case["ragged"])
+        pairs = sum(n * case["past"] + n * (n + 1) // 2 for n in lq)
+        rows_k = sum(lq) + case["past"] * len(lq)
+        return {"bytes": sum(lq) * h * d * 4 + rows_k * g * d * 4 + 8 * len(lq) + 8, "flops": 4.0 * d * h * pairs}
+    each = g * (2 * d if case["type"] == "fp16" else d + 4)   # one cached token's keys, or values
+    if op == "write":
+        return {"bytes": case["rows"] * (4 * g * d + 2 * each + 4), "flops": 0.0}
+    lengths = _lengths(case["seqs"], case["longest"])
+    tables = sum(4 * -(-n // case["page"]) for n in lengths)
+    if op == "read":
+        return {"bytes": sum(lengths) * (2 * each + 4 * g * d) + tables + 4 * len(lengths) + 4, "flops": 0.0}
+    return {"bytes": sum(lengths) * 2 * each + tables + len(lengths) * (4 + 4 * h * d), "flops": 4.0 * d * h * sum(lengths)}
+
+
+# ---- from the definitions, in 64 bits ----------------------------------------------------------
+def exact(case, seed):
+    s = prepare(case, seed)
+    h, g, d = HEADS[case["heads"]]
+    op, dev = case["op"], "cuda"
+    if op == "rope":
+        half, x = case["rot"] // 2, s["x"].double().view(-1, h + 2 * g, d)
+        a = s["pos"].double()[:, None] * torch.tensor([THETA ** (-i / half) for i in range(half)], dtype=torch.float64, device=dev)
+        turn = torch.polar(torch.ones_like(a), a)[:, None]
+        z = torch.complex(x[:, :h + g, :half].contiguous(), x[:, :h + g, half:2 * half].contiguous()) * turn
+        x[:, :h + g, :2 * half] = torch.cat([z.real, z.imag], -1)
+        return x.view(s["x"].shape)
+    if op == "attn":
+        out, cq, ck = [], s["cu_q"].tolist(), s["cu_k"].tolist()
+        for i in range(case["seqs"]):
+            q, k, v = (t[c[i]:c[i + 1]].double() for t, c in ((s["q"], cq), (s["k"], ck), (s["v"], ck)))
+            hidden = torch.ones(len(q), len(k), dtype=torch.bool, device=dev).triu_(len(k) - len(q) + 1)
+            one = torch.empty_like(q)
+            for a in range(h):
+                x = (q[:, a] @ k[:, a // (h // g)].T) / math.sqrt(d)
+                one[:, a] = torch.softmax(x.masked_fill_(hidden, -math.inf), -1) @ v[:, a // (h // g)]
+            out.append(one)
+        return torch.cat(out)
+    if op == "write":
+        kv, slots = s["kv"], s["slot"].tolist()
+        x = s["p16"].double().view(-1, h + 2 * g, d)
+        out, scales = [], []
+        at = torch.tensor([[t // case["page"], t % case["page"]] for t in slots], device=dev)
+        for n, y in (("k", x[:, h:h + g]), ("v", x[:, h + g:])):
+            pool = kv[n].double()
+            if case["type"] == "e4m3":
+                top = y.abs().amax(-1, keepdim=True)
+                scale = torch.exp2(torch.ceil(torch.log2(top / 448.0)))
+                size = torch.floor(torch.log2((y / scale).abs().clamp_min(2.0 ** -6)))   # e4m3: three bits behind the leading one
+                y = torch.round(y / scale * torch.exp2(3.0 - size)) / torch.exp2(3.0 - size)
+                sc = kv[n + "_scale"].double()
+                sc[at[:, 0], :, at[:, 1]] = scale[..., 0]
+                scales.append(sc)
+            pool[at[:, 0], :, at[:, 1]] = y
+            out.append(pool)
+        return out + scales
+    lengths, page = _lengths(case["seqs"], case["longest"]), case["page"]
+    out = ([], []) if op == "read" else []
+    for i, n in enumerate(lengths):
+        pages = s["table"][i, :-(-n // page)].long()
+        rows = []
+        for name in ("k", "v"):
+            x = s["kv"][name].view(torch.uint8)[pages].view(torch.float8_e4m3fn).double() if case["type"] == "e4m3" else s["kv"][name][pages].double()
+            if case["type"] == "e4m3":
+                x = x * s["kv"][name + "_scale"][pages].double()[..., None]
+            rows.append(x.permute(0, 2, 1, 3).reshape(-1, g, d)[:n])
+        if op == "read":
+            out[0].append(rows[0])
+            out[1].append(rows[1])
+        else:
+            q = s["q"][i].double().view(g, h // g, d)
+            x = torch.softmax(torch.einsum("gmd,jgd->gmj", q, rows[0]) / math.sqrt(d), -1)
+            out.append(torch.einsum("gmj,jgd->gmd", x, rows[1]).reshape(1, h, d))
+    return [torch.cat(t) for t in out] if op == "read" else torch.cat(out)
