@@ -198,6 +198,85 @@ void moe_cuda_hc(moe_cuda_ctx_t *c, const float *a, const float *b, float *h, st
 void moe_cuda_dense(moe_cuda_ctx_t *c, const void *A16, const void *W, float *C, const uint32_t *amax,
                     struct moe_pc_dense_t pc);
 
+/* ---- the attention half of a layer ------------------------------------------
+ * What stands between the projection of a layer's input (moe_cuda_dense: queries,
+ * keys and values of a row side by side, fp32) and its output projection
+ * (moe_cuda_dense again): rotary positions, a paged key-value cache, attention
+ * over whole prompts and of one new token over the cache.  The teacher's own
+ * form of it is a plain causal softmax per head (shader/qwen_attn.comp).
+ * host/moe_attn.c composes the calls.
+ *
+ * Operands are fp16 at 16-byte addresses, rows at strides that are multiples of
+ * 8 elements; sums, softmax statistics and angles are fp32 or wider.  A group of
+ * heads / kv_heads query heads shares a key-value head: query head j reads head
+ * j / (heads / kv_heads).  A call on a context whose device is not the current
+ * one runs on the context's device.  None of them allocates, so all of them can
+ * be captured into a graph; the attentions use the context's work area, so
+ * graphs captured from one context must not run at the same time.
+ * Sizes that the host knows are refused with MOE_ERR_ARG before anything runs.
+ * What only the device can see (a slot, page or length out of its range) is
+ * skipped without an access, and the status becomes MOE_ERR_ARG by the next
+ * flush. */
+
+/* Rotary positions, and the fp32 -> fp16 rounding of all three operands: x fp32
+ * [rows x stride], per row `heads` heads of hd columns (queries, keys, values in
+ * turn).  In the first rot_heads heads the pairs (i, i + rot/2), i < rot/2, turn
+ * by pos[row] * theta^(-2i/rot), the angle taken in 64 bits; all other columns
+ * are only rounded.  out [rows x out_stride] fp16.  pos may be NULL if rot_heads
+ * is 0.  hd % 8 == 0, rot % 8 == 0, rot <= hd, rot <= 512; stride % 4 == 0. */
+struct moe_pc_rope_t { uint32_t rows, heads, rot_heads, hd, rot, stride, out_stride; float theta; };
+void moe_cuda_rope(moe_cuda_ctx_t *c, const float *x, const uint32_t *pos, void *out, struct moe_pc_rope_t pc);
+
+/* A paged cache of one layer.  k and v: [pages][kv_heads][page][hd]; place p of
+ * page g is slot g * page + p.  MOE_KV_E4M3 holds 8-bit floats (e4m3) and, for
+ * every slot and kv head, one positive scale each for keys and values
+ * ([pages][kv_heads][page] fp32): value = code * scale.  hd 64 or 128; page a power of two
+ * from 16 to 256; fewer than 2^32 - 1 slots. */
+typedef struct moe_cuda_kv_t {
+    void *k, *v;
+    float *k_scale, *v_scale; /* MOE_KV_E4M3 only */
+    uint32_t pages, page, kv_heads, hd, type;
+} moe_cuda_kv_t;
+#define MOE_KV_F16 0u
+#define MOE_KV_E4M3 1u
+
+/* rows of k16 and v16 ([rows x stride], kv_heads * hd columns used) into the
+ * slots slot[row] (MDA_PC_NO_SLOT: this row is not kept).  e4m3: the scale is the
+ * least power of two with amax <= 448 * scale (1 for zeros), so that reading back
+ * to fp16 is exact for normal fp16 values; rounding to nearest even; a NaN stays
+ * NaN and does not enter amax; infinities count as 65504 there and read back as
+ * infinities.  Two rows with one slot: either may be kept, head by head. */
+struct moe_pc_kv_write_t { uint32_t rows, stride; };
+void moe_cuda_kv_write(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const void *k16, const void *v16, const uint32_t *slot,
+                       struct moe_pc_kv_write_t pc);
+
+/* Back out of the cache, as moe_cuda_attn takes them: rows cu[s] .. cu[s+1]-1 of
+ * k16 and v16 ([rows x stride]) become places 0, 1, ... of sequence s, whose
+ * pages are table[s * table_stride + place / page].  cu[seqs + 1] never falls;
+ * rows from cu[seqs] on, and rows whose page is refused, are left as they were. */
+struct moe_pc_kv_read_t { uint32_t seqs, rows, table_stride, stride; };
+void moe_cuda_kv_read(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const uint32_t *table, const uint32_t *cu, void *k16, void *v16,
+                      struct moe_pc_kv_read_t pc);
+
+/* Causal attention over packed prompts.  Sequence s has query rows cu_q[s] ..
+ * cu_q[s+1]-1 and key rows cu_k[s] .. cu_k[s+1]-1 (lengths lq, lk); its query i
+ * sees keys 0 .. i + lk - lq.  o = softmax(scale * q k^T) v per head; a query that
+ * sees nothing gives 0; keys and values that a query does not see do not matter to
+ * it, whatever they hold.  Output rows behind cu_q[seqs] are left as they were.
+ * hd 64 or 128; heads / kv_heads from 1 to 16; row counts below 2^31. */
+struct moe_pc_attn_t { uint32_t seqs, rows_q, rows_k, heads, kv_heads, hd, q_stride, kv_stride, o_stride; float scale; };
+void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k16, const void *v16, const uint32_t *cu_q, const uint32_t *cu_k,
+                   void *o16, struct moe_pc_attn_t pc);
+
+/* Attention of one new token per sequence over the cache: query row s sees places
+ * 0 .. len[s]-1 of sequence s (its own key and value have been written before).
+ * len[s] == 0 gives 0.  max_len bounds len[] (a longer one is refused on the
+ * device: that sequence gives 0); the work is divided by the lengths themselves.
+ * Places on a refused page count as not there. */
+struct moe_pc_attn_decode_t { uint32_t seqs, heads, max_len, table_stride, q_stride, o_stride; float scale; };
+void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const void *q16, const uint32_t *table, const uint32_t *len,
+                          void *o16, struct moe_pc_attn_decode_t pc);
+
 /* ---- weight upload step ---------------------------------------------------
  * shader/qwen_bf16.comp (binding w; call mda_qwen_convert, src/qwen.c:365-378):
  * pc.n 32-bit words of two bf16 values each, rewritten in place as fp16 (round

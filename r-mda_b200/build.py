@@ -25,7 +25,7 @@ def _stale(target: str, sources: list[str]) -> bool:
 
 def build_cuda(force: bool = False, verbose: bool = False) -> str:
     srcs = sorted(glob.glob(os.path.join(PKG, "csrc", "*.cu")))
-    deps = srcs + glob.glob(os.path.join(PKG, "csrc", "*.cuh")) + [os.path.join(ROOT, "include", "moe_cuda.h")]
+    deps = srcs + glob.glob(os.path.join(PKG, "csrc", "*.cuh")) + glob.glob(os.path.join(PKG, "csrc", "*.h")) + [os.path.join(ROOT, "include", "moe_cuda.h")]
     if force or _stale(LIB, deps):
         cmd = ["nvcc"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB] + srcs + ["-ldl"]
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,0 +1,37 @@
+// What the attention calls share: refusals, the device-side refusal, the context's device, small conversions.
+#pragma once
+
+#include "moe_attn_args.h"
+#include "moe_common.cuh"
+
+// Kinds of device-side refusals (MOE_ERR_ARG | kind << 8 in the status word).
+enum { MOE_SITE_SLOT = 1, MOE_SITE_PAGE = 2, MOE_SITE_LENGTH = 3, MOE_SITE_ROWS = 4 };
+
+// The calling thread's current device is the context's for as long as this lives.
+struct moe_on_device {
+    int before;
+    bool moved;
+    explicit moe_on_device(const moe_cuda_ctx *c) : before(0), moved(false) {
+        if (cudaGetDevice(&before) == cudaSuccess && before != c->device) moved = cudaSetDevice(c->device) == cudaSuccess;
+    }
+    ~moe_on_device() {
+        if (moved) (void)cudaSetDevice(before);
+    }
+    moe_on_device(const moe_on_device &) = delete;
+    moe_on_device &operator=(const moe_on_device &) = delete;
+};
+
+static inline uint32_t moe_log2(uint32_t power_of_two) {
+    uint32_t n = 0;
+    while ((1u << n) < power_of_two) n += 1;
+    return n;
+}
+
+__device__ __forceinline__ void moe_deny(uint32_t *status, uint32_t kind) { atomicCAS(status, 0u, (uint32_t)MOE_ERR_ARG | (kind << 8)); }
+
+// Two e4m3 codes (low 16 bits) as two fp16 values; exact, NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t codes) {
+    uint32_t h2;
+    asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}\n" : "=r"(h2) : "r"(codes));
+    return h2;
+}

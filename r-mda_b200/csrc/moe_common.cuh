@@ -74,6 +74,7 @@ struct moe_cuda_ctx {
     int fail_alloc_countdown;
     bool mm_attr_set[4];
     bool kd_attr_set;
+    bool dec_attr_set[8], attn_attr_set[4];
     uint32_t *ticket;  // device word, zero between kernels: "last block done" counter
     bool sw_attr_set[8];
     moe_ep_state *ep;

@@ -28,6 +28,10 @@ bool moe_poll_device_status(moe_cuda_ctx *c) {
                 moe_fail(c, code, "route: row %u has fewer selectable logits than topk", w >> 8);
             } else if (code == MOE_ERR_TIMEOUT) {
                 moe_fail(c, code, "device wait gave up (site %u)", w >> 8);
+            } else if (code == MOE_ERR_ARG) {
+                static const char *const what[] = {"argument", "cache slot", "page or place", "sequence length", "row range"};
+                const uint32_t kind = w >> 8;
+                moe_fail(c, code, "attention: a %s on the device is outside its range", what[kind < 5u ? kind : 0u]);
             } else {
                 moe_fail(c, code, "device reported status 0x%x", w);
             }

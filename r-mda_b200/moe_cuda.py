@@ -14,6 +14,7 @@ NO_SLOT = 0xFFFFFFFF
 TILE = 128
 MOE_OK, MOE_ERR_CUDA, MOE_ERR_ARG, MOE_ERR_NOMEM, MOE_ERR_ROUTE, MOE_ERR_TIMEOUT, MOE_ERR_COMM, MOE_ERR_UNSUPPORTED = range(8)
 LAYER_UNFUSED, LAYER_YE_F32, LAYER_CHUNKED, LAYER_NO_PAIR, LAYER_MATERIALIZE_XP, LAYER_TILED = 1, 2, 4, 8, 16, 32
+KV_F16, KV_E4M3 = 0, 1
 PROF_STAGES = ("route", "scan", "scatter", "gate_up", "down", "shared", "combine")
 
 
@@ -67,6 +68,32 @@ class PcDense(C.Structure):
 
 class PcKd(C.Structure):
     _fields_ = [("rows", C.c_uint32), ("vocab", C.c_uint32)]
+
+
+class PcRope(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("rows", "heads", "rot_heads", "hd", "rot", "stride", "out_stride")] + [("theta", C.c_float)]
+
+
+class Kv(C.Structure):
+    """moe_cuda_kv_t: a paged key-value cache; pointers are DevBufs' or raw device addresses."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [(n, C.c_uint32) for n in ("pages", "page", "kv_heads", "hd", "type")]
+
+
+class PcKvWrite(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("stride", C.c_uint32)]
+
+
+class PcKvRead(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("seqs", "rows", "table_stride", "stride")]
+
+
+class PcAttn(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("seqs", "rows_q", "rows_k", "heads", "kv_heads", "hd", "q_stride", "kv_stride", "o_stride")]
+                + [("scale", C.c_float)])
+
+
+class PcAttnDecode(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("seqs", "heads", "max_len", "table_stride", "q_stride", "o_stride")] + [("scale", C.c_float)]
 
 
 class Layer(C.Structure):
@@ -138,6 +165,11 @@ def lib() -> C.CDLL:
         L.moe_cuda_norm.argtypes = [vp, vp, vp, vp, vp, PcNorm]
         L.moe_cuda_hc.argtypes = [vp, vp, vp, vp, PcHc]
         L.moe_cuda_dense.argtypes = [vp, vp, vp, vp, vp, PcDense]
+        L.moe_cuda_rope.argtypes = [vp, vp, vp, vp, PcRope]
+        L.moe_cuda_kv_write.argtypes = [vp, C.POINTER(Kv), vp, vp, vp, PcKvWrite]
+        L.moe_cuda_kv_read.argtypes = [vp, C.POINTER(Kv), vp, vp, vp, vp, PcKvRead]
+        L.moe_cuda_attn.argtypes = [vp, vp, vp, vp, vp, vp, vp, PcAttn]
+        L.moe_cuda_attn_decode.argtypes = [vp, C.POINTER(Kv), vp, vp, vp, vp, PcAttnDecode]
         L.moe_cuda_moe_rows.restype = u32
         L.moe_cuda_moe_rows.argtypes = [u32, u32, u32]
         L.moe_cuda_layer.argtypes = [vp, C.POINTER(Layer)]
@@ -306,6 +338,33 @@ class Ctx:
 
     def kd_bytes(self, logits, toks, cont, outp, rows, vocab):
         lib().moe_cuda_kd_bytes(self.p, _ptr(logits), _ptr(toks), _ptr(cont), _ptr(outp), PcKd(rows, vocab))
+
+    # ---- the attention half of a layer; strides default to rows without gaps ----
+    def rope(self, x, pos, out, rows, heads, rot_heads, hd, rot, theta, stride=None, out_stride=None):
+        n = heads * hd
+        lib().moe_cuda_rope(self.p, _ptr(x), _ptr(pos), _ptr(out), PcRope(rows, heads, rot_heads, hd, rot, n if stride is None else stride,
+                                                                          n if out_stride is None else out_stride, theta))
+
+    def kv_write(self, kv, k16, v16, slot, rows, stride=None):
+        lib().moe_cuda_kv_write(self.p, C.byref(kv), _ptr(k16), _ptr(v16), _ptr(slot),
+                                PcKvWrite(rows, kv.kv_heads * kv.hd if stride is None else stride))
+
+    def kv_read(self, kv, table, cu, k16, v16, seqs, rows, table_stride, stride=None):
+        lib().moe_cuda_kv_read(self.p, C.byref(kv), _ptr(table), _ptr(cu), _ptr(k16), _ptr(v16),
+                               PcKvRead(seqs, rows, table_stride, kv.kv_heads * kv.hd if stride is None else stride))
+
+    def attn(self, q16, k16, v16, cu_q, cu_k, o16, seqs, rows_q, rows_k, heads, kv_heads, hd, q_stride=None, kv_stride=None, o_stride=None,
+             scale=None):
+        pc = PcAttn(seqs, rows_q, rows_k, heads, kv_heads, hd, heads * hd if q_stride is None else q_stride,
+                    kv_heads * hd if kv_stride is None else kv_stride, heads * hd if o_stride is None else o_stride,
+                    hd ** -0.5 if scale is None else scale)
+        lib().moe_cuda_attn(self.p, _ptr(q16), _ptr(k16), _ptr(v16), _ptr(cu_q), _ptr(cu_k), _ptr(o16), pc)
+
+    def attn_decode(self, kv, q16, table, length, o16, seqs, heads, max_len, table_stride, q_stride=None, o_stride=None, scale=None):
+        n = heads * kv.hd
+        pc = PcAttnDecode(seqs, heads, max_len, table_stride, n if q_stride is None else q_stride, n if o_stride is None else o_stride,
+                          kv.hd ** -0.5 if scale is None else scale)
+        lib().moe_cuda_attn_decode(self.p, C.byref(kv), _ptr(q16), _ptr(table), _ptr(length), _ptr(o16), pc)
 
     def layer(self, **kw):
         L = Layer()

@@ -1,0 +1,380 @@
+"""The attention half of a layer against plain 64-bit forms: rotary positions, the paged key-value cache (fp16 and e4m3),
+attention over packed prompts and of one new token over the cache, alone and together."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from . import attn_ref as R
+
+pytestmark = pytest.mark.gpu
+NO_SLOT = 0xFFFFFFFF
+
+
+@pytest.fixture()
+def on(mc):
+    """A context on a torch stream that is current for the test."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = mc.Ctx(0, stream.cuda_stream)
+        c.check()
+        yield c
+        torch.cuda.synchronize()
+        c.close()
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _f16(gen, *shape):
+    return torch.randn(shape, device="cuda", generator=gen).half()
+
+
+def _u32(values):
+    return torch.from_numpy(np.asarray(values, dtype=np.uint32).view(np.int32)).cuda()
+
+
+def _starts(lengths):
+    return _u32(np.concatenate([[0], np.cumsum(lengths)]))
+
+
+# ---- rotary positions ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,heads,rot_heads,hd,rot,theta,gap", [
+    (1, 1, 1, 64, 64, 1e4, 0), (37, 6, 4, 128, 128, 1e6, 8), (5, 40, 36, 128, 64, 1e6, 0), (300, 20, 16, 64, 48, 5e5, 16),
+    (1201, 3, 3, 8, 8, 1e4, 0), (3, 5, 0, 64, 0, 0.0, 0), (9, 2, 1, 512, 512, 1e7, 8)])
+def test_rope(on, rows, heads, rot_heads, hd, rot, theta, gap):
+    g = _gen(rows)
+    n = heads * hd
+    x = torch.randn(rows, n + gap, device="cuda", generator=g) * 3
+    pos = torch.randint(0, 2 ** 20, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    pos[0] = 0
+    if rows > 4:
+        pos[3], pos[4] = -1, 2 ** 31 - 1   # the largest unsigned position
+    out = torch.full((rows + 1, n + 2 * gap), 7.0, device="cuda", dtype=torch.float16)
+    on.rope(x.data_ptr(), pos.data_ptr() if rot_heads else None, out.data_ptr(), rows, heads, rot_heads, hd, rot, theta, n + gap, n + 2 * gap)
+    on.flush()
+    z = x[:, :n].double().view(rows, heads, hd)
+    ref, err = z.clone(), torch.zeros_like(z)
+    if rot_heads:
+        half = rot // 2
+        a = (pos.long() & 0xFFFFFFFF).double()[:, None] * torch.tensor([float(np.float32(theta)) ** (-i / half) for i in range(half)], device="cuda", dtype=torch.float64)
+        c, s = a.cos()[:, None], a.sin()[:, None]
+        lo, hi = z[:, :rot_heads, :half], z[:, :rot_heads, half:rot]
+        ref[:, :rot_heads, :half], ref[:, :rot_heads, half:rot] = lo * c - hi * s, hi * c + lo * s
+        # sines: the turn's fraction rounds to 24 bits (pi * 2^-24 of angle), 64-bit products of positions up to 2^32 and
+        # frequencies with some steps of 2^-53 each (2^32 * 2^-50 * 2 pi), two steps of the function itself; three fp32 roundings
+        err[:, :rot_heads, :half] = err[:, :rot_heads, half:rot] = (lo.abs() + hi.abs()) * (math.pi * 2.0 ** -24 + math.pi * 2.0 ** -17 * 0.5 + 5 * 2.0 ** -24)
+    got = out[:rows, :n].double().view(rows, heads, hd)
+    assert ((got - ref).abs() <= ref.abs() * 2.0 ** -11 + 2.0 ** -25 + err * 1.01).all()
+    assert (out[rows:] == 7).all() and (out[:, n:] == 7).all()
+
+
+def test_rope_far_positions_are_exact_to_fp16(on):
+    """Positions up to 2^20 with the plain bound (no allowance for a position times a frequency)."""
+    rows, hd = 512, 128
+    g = _gen(1)
+    x = torch.randn(rows, hd, device="cuda", generator=g)
+    pos = torch.randint(2 ** 19, 2 ** 20, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    out = torch.empty(rows, hd, device="cuda", dtype=torch.float16)
+    on.rope(x.data_ptr(), pos.data_ptr(), out.data_ptr(), rows, 1, 1, hd, hd, 10000.0)
+    on.flush()
+    a = pos.double()[:, None] * torch.tensor([10000.0 ** (-i / 64) for i in range(64)], device="cuda", dtype=torch.float64)
+    lo, hi = x[:, :64].double(), x[:, 64:].double()
+    ref = torch.cat([lo * a.cos() - hi * a.sin(), hi * a.cos() + lo * a.sin()], 1)
+    far = (lo.abs() + hi.abs()).repeat(1, 2)
+    assert ((out.double() - ref).abs() <= ref.abs() * 2.0 ** -11 + 2.0 ** -25 + far * 1e-6).all()
+
+
+# ---- the cache ----------------------------------------------------------------------------------
+class Cache:
+    def __init__(self, mc, gen, pages, page, heads, hd, e4m3, fill=None):
+        self.page, self.heads, self.hd, self.e4m3 = page, heads, hd, e4m3
+        shape = (pages, heads, page, hd)
+        x = [_f16(gen, *shape) for _ in range(2)] if fill is None else [torch.full(shape, fill, device="cuda", dtype=torch.float16) for _ in range(2)]
+        self.scales = None
+        if e4m3:
+            (self.k, ks), (self.v, vs) = (R.e4m3(t * torch.exp2(torch.randint(-6, 6, t.shape[:3], device="cuda", generator=gen).float())[..., None].half()) for t in x)
+            self.scales = [ks.contiguous(), vs.contiguous()]
+        else:
+            self.k, self.v = x
+        at = [t.data_ptr() for t in self.scales] if e4m3 else [None, None]
+        self.c = mc.Kv(k=self.k.data_ptr(), v=self.v.data_ptr(), k_scale=at[0], v_scale=at[1], pages=pages, page=page, kv_heads=heads, hd=hd,
+                       type=mc.KV_E4M3 if e4m3 else mc.KV_F16)
+
+    def rows(self, pages, n):
+        """The first n tokens on these pages, [n, heads, hd] in float64."""
+        out = []
+        for i, t in enumerate((self.k, self.v)):
+            x = t.view(torch.uint8)[pages].view(torch.float8_e4m3fn).double() if self.e4m3 else t[pages].double()
+            if self.e4m3:
+                x = x * self.scales[i][pages].double()[..., None]
+            out.append(x.transpose(1, 2).reshape(-1, self.heads, self.hd)[:n])
+        return out
+
+
+def _table(gen, lengths, page, pages, stride):
+    order = torch.randperm(pages, device="cuda", generator=gen).int()
+    table = torch.full((len(lengths), stride), 0x7FFFFFFF, device="cuda", dtype=torch.int32)   # unused entries are never looked at
+    at = 0
+    for i, n in enumerate(lengths):
+        m = -(-n // page)
+        table[i, :m] = order[at:at + m]
+        at += m
+    return table
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("rows,heads,hd,page,gap", [(1, 1, 64, 16, 0), (7, 4, 128, 64, 640), (129, 3, 128, 16, 0), (1000, 2, 64, 256, 8), (4099, 16, 128, 32, 8)])
+def test_kv_write(on, mc, e4m3, rows, heads, hd, page, gap):
+    g = _gen(rows + heads)
+    pages = -(-rows // page) + 2
+    kv = Cache(mc, g, pages, page, heads, hd, e4m3)
+    stride = heads * hd + gap
+    k, v = _f16(g, rows, stride), _f16(g, rows, stride)
+    for t in (k, v):
+        t *= torch.exp2(torch.randint(-14, 9, (rows, 1), device="cuda", generator=g).float()).half()
+    k[0, :hd] = 0
+    v[0, 0] = 65504
+    k[rows // 2, 1] = 448 * 2.0 ** -12   # exactly a scale's largest value
+    slot = torch.randperm(pages * page, device="cuda", generator=g)[:rows].int()
+    if rows > 2:
+        slot[1] = -1   # not kept
+    want = [t.clone().view(torch.uint8 if e4m3 else torch.float16) for t in (kv.k, kv.v)]
+    scales = [t.clone() for t in kv.scales] if e4m3 else None
+    on.kv_write(kv.c, k.data_ptr(), v.data_ptr(), slot.data_ptr(), rows, stride)
+    on.flush()
+    kept = slot >= 0
+    at = slot[kept].long()
+    for i, t in enumerate((k, v)):
+        x = t[kept, :heads * hd].view(-1, heads, hd)
+        if e4m3:
+            code, scale = R.e4m3(x)
+            want[i][at // page, :, at % page] = code.view(torch.uint8)
+            scales[i][at // page, :, at % page] = scale
+            assert torch.equal(kv.scales[i], scales[i])
+            assert torch.equal((kv.k, kv.v)[i].view(torch.uint8), want[i])
+        else:
+            want[i][at // page, :, at % page] = x
+            assert torch.equal((kv.k, kv.v)[i], want[i])
+
+
+def test_kv_write_special_values_and_back(on, mc):
+    """NaN, infinities, zeros and subnormals through an e4m3 cache and back."""
+    g = _gen(3)
+    kv = Cache(mc, g, 1, 16, 1, 64, True)
+    x = torch.zeros(6, 64, device="cuda", dtype=torch.float16)
+    x[0, 3], x[0, 4] = float("nan"), 1.5
+    x[1, 0], x[1, 1], x[1, 2] = float("inf"), -float("inf"), 300.0
+    x[2, 5] = 2.0 ** -24
+    x[3] = -0.0
+    x[4, :3] = torch.tensor([448.0, 17.0, 2.0 ** -9], device="cuda")
+    x[5, :] = float("nan")
+    slot, cu, table = _u32(range(6)), _u32([0, 6]), _u32([0])
+    k, v = torch.empty_like(x), torch.empty_like(x)
+    on.kv_write(kv.c, x.data_ptr(), x.data_ptr(), slot.data_ptr(), 6)
+    on.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), 1, 6, 1)
+    on.flush()
+    assert torch.equal(k.view(torch.int16), v.view(torch.int16))
+    assert torch.isnan(k[0, 3]) and k[0, 4] == 1.5 and k[0, 0] == 0
+    assert k[1, 0] == float("inf") and k[1, 1] == -float("inf") and k[1, 2] == 288   # 300 / 256 = 1.171875 to four bits: 1.125
+    assert k[2, 5] == 2.0 ** -24 and (k[3] == 0).all() and torch.isnan(k[5]).all()
+    assert k[4, 0] == 448 and k[4, 1] == 16   # 17 lies half way between 16 and 18: the even one
+    code, scale = R.e4m3(x)
+    want = (code.float() * scale[..., None]).half()
+    assert torch.equal(torch.nan_to_num(k, nan=7.0)[2:], torch.nan_to_num(want, nan=7.0)[2:])
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,heads,hd,page,gap", [([1], 1, 64, 16, 0), ([0, 5, 0, 33, 16, 0], 4, 128, 16, 8), ([513, 1, 700], 2, 64, 256, 0),
+                                                        ([64] * 40, 16, 128, 64, 0), ([3000], 8, 128, 32, 24)])
+def test_kv_read(on, mc, e4m3, lengths, heads, hd, page, gap):
+    g = _gen(sum(lengths))
+    need = sum(-(-n // page) for n in lengths)
+    kv = Cache(mc, g, need + 1, page, heads, hd, e4m3)
+    per = max(1, max(-(-n // page) for n in lengths))
+    table = _table(g, lengths, page, need + 1, per)
+    total, stride = sum(lengths), heads * hd + gap
+    k, v = (torch.full((total + 2, stride), 7.0, device="cuda", dtype=torch.float16) for _ in range(2))
+    cu = _starts(lengths)
+    on.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), len(lengths), total + 2, per, stride)
+    on.flush()
+    at = 0
+    for i, n in enumerate(lengths):
+        rk, rv = kv.rows(table[i, :-(-n // page)].long(), n)
+        assert torch.equal(k[at:at + n, :heads * hd].view(n, heads, hd), rk.half())
+        assert torch.equal(v[at:at + n, :heads * hd].view(n, heads, hd), rv.half())
+        at += n
+    assert (k[total:] == 7).all() and (k[:, heads * hd:] == 7).all() and (v[total:] == 7).all()
+
+
+# ---- one new token over the cache ----------------------------------------------------------------
+def _decode(on, mc, g, lengths, heads, kv_heads, hd, page, e4m3, gap=0, poison=True, max_len=None):
+    need = sum(-(-n // page) for n in lengths)
+    kv = Cache(mc, g, need + 1, page, kv_heads, hd, e4m3)
+    per = max(1, max(-(-n // page) for n in lengths))
+    table = _table(g, lengths, page, need + 1, per)
+    rows = [kv.rows(table[i, :-(-n // page)].long(), n) for i, n in enumerate(lengths)]
+    if poison:   # what lies behind a sequence's last token on its last page is nobody's
+        for i, n in enumerate(lengths):
+            if n % page:
+                last = int(table[i, n // page])
+                for j, t in enumerate((kv.k, kv.v)):
+                    t[last, :, n % page:] = float("nan")
+                    if e4m3:
+                        kv.scales[j][last, :, n % page:] = float("inf") if j else float("nan")
+    seqs, length = len(lengths), _u32(lengths)
+    q = _f16(g, seqs, heads * hd + gap)
+    out = torch.full((seqs + 1, heads * hd + 2 * gap), 7.0, device="cuda", dtype=torch.float16)
+    on.attn_decode(kv.c, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), seqs, heads,
+                   max(lengths) if max_len is None else max_len, per, heads * hd + gap, heads * hd + 2 * gap)
+    on.flush()
+    assert (out[seqs:] == 7).all() and (out[:, heads * hd:] == 7).all()
+    for i, n in enumerate(lengths):
+        got = out[i:i + 1, :heads * hd].view(1, heads, hd)
+        if n == 0:
+            assert (got == 0).all()
+            continue
+        o, mass, size = R.attention(q[i:i + 1, :heads * hd].double().view(1, heads, hd), *rows[i], hd ** -0.5, n - 1)
+        R.check(got, o, mass, size, hd, n)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lengths,heads,kv_heads,page", [
+    ([1], 1, 1, 16), ([0, 1, 0], 8, 1, 16), ([15, 16, 17, 31, 32, 33, 0, 63, 64, 65], 8, 2, 16), ([777], 32, 4, 64),
+    ([5, 1000, 3, 129, 0, 0, 512], 14, 2, 32), ([2049] * 3, 16, 1, 128), ([100, 3000], 10, 10, 256), ([33] * 300, 6, 2, 16)])
+def test_decode(on, mc, e4m3, hd, lengths, heads, kv_heads, page):
+    _decode(on, mc, _gen(len(lengths) + heads), lengths, heads, kv_heads, hd, page, e4m3)
+
+
+def test_decode_strides_and_a_loose_bound(on, mc):
+    _decode(on, mc, _gen(9), [40, 7, 100], 12, 4, 64, 16, False, gap=24, max_len=112)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_decode_long(on, mc, e4m3):
+    """One long sequence on the whole chip, several pieces to every head."""
+    _decode(on, mc, _gen(4), [100003, 3], 8, 1, 128, 64, e4m3)
+
+
+def test_decode_far_offsets(on, mc):
+    """Pages beyond 2^32 elements of the pool."""
+    pages, page, heads, hd = 34000, 256, 4, 128   # 4.46e9 elements each
+    k = torch.empty(pages, heads, page, hd, device="cuda", dtype=torch.float16)
+    v = torch.empty_like(k)
+    g = _gen(5)
+    table = torch.tensor([[33999, 3, 33000]], device="cuda", dtype=torch.int32)
+    for t in (k, v):
+        for p in table[0].tolist():
+            t[p] = _f16(g, heads, page, hd)
+    kv = mc.Kv(k=k.data_ptr(), v=v.data_ptr(), k_scale=None, v_scale=None, pages=pages, page=page, kv_heads=heads, hd=hd, type=mc.KV_F16)
+    n = 700
+    row = _f16(g, 2, heads * hd)
+    slot = _u32([33000 * 256 + 187, 33999 * 256])   # places 699 and 0
+    length, cu = _u32([n]), _u32([0, n])
+    on.kv_write(kv, row.data_ptr(), row.data_ptr(), slot.data_ptr(), 2)
+    q, out = _f16(g, 1, 8 * hd), torch.empty(1, 8 * hd, device="cuda", dtype=torch.float16)
+    on.attn_decode(kv, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), 1, 8, n, 3)
+    kr, vr = torch.empty(n, heads, hd, device="cuda", dtype=torch.float16), torch.empty(n, heads, hd, device="cuda", dtype=torch.float16)
+    on.kv_read(kv, table.data_ptr(), cu.data_ptr(), kr.data_ptr(), vr.data_ptr(), 1, n, 3)
+    on.flush()
+    x = [t[table[0].long()].transpose(1, 2).reshape(-1, heads, hd)[:n] for t in (k, v)]
+    assert torch.equal(x[0][699].flatten(), row[0]) and torch.equal(x[0][0].flatten(), row[1])
+    assert torch.equal(kr, x[0]) and torch.equal(vr, x[1])
+    o, mass, size = R.attention(q.double().view(1, 8, hd), x[0].double(), x[1].double(), hd ** -0.5, n - 1)
+    R.check(out.view(1, 8, hd), o, mass, size, hd, n)
+
+
+def test_decode_large_logits_and_wide_scales(on, mc):
+    """Logits far apart, V scales from 2^-20 to 2^6: the rows that carry the weight are the small ones."""
+    g = _gen(6)
+    n, hd = 200, 64
+    kv = Cache(mc, g, 13, 16, 1, hd, True)
+    order = torch.arange(13, device="cuda", dtype=torch.int32)[None].contiguous()
+    kv.scales[1][:] = 2.0 ** -20
+    kv.scales[1][0, 0, 3] = 2.0 ** 6
+    kv.scales[0][:] = 2.0 ** -4
+    q, length = _f16(g, 1, 4 * hd) * 8, _u32([n])
+    rows = kv.rows(order[0].long(), n)
+    out = torch.empty(1, 4 * hd, device="cuda", dtype=torch.float16)
+    on.attn_decode(kv.c, q.data_ptr(), order.data_ptr(), length.data_ptr(), out.data_ptr(), 1, 4, n, 13)
+    on.flush()
+    o, mass, size = R.attention(q.double().view(1, 4, hd), *rows, hd ** -0.5, n - 1)
+    R.check(out.view(1, 4, hd), o, mass, size, hd, n)
+
+
+# ---- whole prompts --------------------------------------------------------------------------------
+def _attn(on, g, lq, lk, heads, kv_heads, hd, gap=0, poison=False, scale=None):
+    nq, nk = sum(lq), sum(lk)
+    q, k, v = _f16(g, nq + 1, heads * hd + gap), _f16(g, nk + 1, kv_heads * hd + gap), _f16(g, nk + 1, kv_heads * hd + gap)
+    out = torch.full((nq + 1, heads * hd + 2 * gap), 7.0, device="cuda", dtype=torch.float16)
+    cq, ck = np.concatenate([[0], np.cumsum(lq)]), np.concatenate([[0], np.cumsum(lk)])
+    if poison:
+        # the last third of every other sequence's keys and values is NaN or infinite: rows before it must not notice
+        for i in range(0, len(lq), 2):
+            a, b = ck[i] + lk[i] - lk[i] // 3, ck[i + 1]
+            k[a:b] = float("nan")
+            v[a:b:2] = float("inf")
+            v[a + 1:b:2] = float("nan")
+    k[nk], v[nk] = float("nan"), float("nan")   # behind the last sequence
+    scale = hd ** -0.5 if scale is None else scale
+    cu_q, cu_k = _u32(cq), _u32(ck)
+    on.attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), len(lq), nq, nk, heads, kv_heads,
+            hd, heads * hd + gap, kv_heads * hd + gap, heads * hd + 2 * gap, scale)
+    on.flush()
+    assert (out[nq:] == 7).all() and (out[:, heads * hd:] == 7).all()
+    for i in range(len(lq)):
+        m = lq[i]
+        clean = m
+        if poison and i % 2 == 0:
+            clean = max(0, min(m, m - lk[i] // 3))   # query r sees keys up to r + lk - lq
+        got = out[cq[i]:cq[i] + m, :heads * hd].view(m, heads, hd)
+        qq = q[cq[i]:cq[i] + m, :heads * hd].double().view(m, heads, hd)
+        kk, vv = (t[ck[i]:ck[i + 1], :kv_heads * hd].double().view(lk[i], kv_heads, hd) for t in (k, v))
+        if poison and i % 2 == 0 and clean < m:
+            assert torch.isnan(got[clean:]).any(-1).all()
+        if clean:
+            cut = clean + lk[i] - m   # keys that any clean query sees
+            o, mass, size = R.attention(qq[:clean], kk[:max(cut, 0)], vv[:max(cut, 0)], scale, lk[i] - m)
+            empty = max(0, min(clean, m - lk[i]))
+            assert (got[:empty] == 0).all()
+            if empty < clean:
+                R.check(got[empty:clean], o[empty:], mass[empty:], size[empty:], hd, lk[i])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lq,lk,heads,kv_heads", [
+    ([1], [1], 1, 1), ([5], [5], 8, 1), ([128], [128], 4, 4), ([129, 1, 127], [129, 1, 127], 6, 2), ([300], [300], 16, 1),
+    ([0, 3, 0, 200, 0], [0, 3, 0, 200, 0], 14, 2), ([64, 65], [500, 1065], 8, 8), ([7, 1, 1], [1000, 1, 513], 12, 4),
+    ([40, 200, 10], [0, 13, 9], 4, 2), ([384] * 5, [384] * 5, 16, 2), ([1100], [1100], 5, 1), ([513, 2, 1000], [600, 300, 1000], 10, 2)])
+def test_attn(on, hd, lq, lk, heads, kv_heads):
+    _attn(on, _gen(sum(lq) + heads), lq, lk, heads, kv_heads, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 1), (4, 4), (14, 2)])
+def test_attn_masked_places_may_hold_anything(on, hd, heads, kv_heads):
+    _attn(on, _gen(heads), [200, 33, 400, 64, 7], [200, 33, 777, 64, 300], heads, kv_heads, hd, poison=True)
+
+
+def test_attn_strides(on):
+    _attn(on, _gen(1), [50, 129], [70, 129], 6, 3, 64, gap=40)
+    _attn(on, _gen(2), [50, 129], [70, 129], 4, 1, 128, gap=8)
+
+
+@pytest.mark.parametrize("scale", [4.0, 1e-3])
+def test_attn_scales(on, scale):
+    """Logits up to several hundred apart, and next to equal ones."""
+    _attn(on, _gen(3), [300], [300], 4, 2, 64, scale=scale)
+
+
+def test_attn_many_sequences(on):
+    rng = np.random.default_rng(0)
+    lq = rng.integers(0, 40, 700).tolist()
+    _attn(on, _gen(4), lq, [n + int(e) for n, e in zip(lq, rng.integers(0, 30, 700))], 4, 2, 64)
+
+
+def test_attn_long(on):
+    _attn(on, _gen(5), [5000], [6001], 8, 2, 128)
