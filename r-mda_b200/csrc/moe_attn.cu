@@ -1,63 +1,665 @@
-// Causal attention over packed prompts: one warp per (query row, head), keys in lanes.  The plain kernel.
+// Causal attention over packed prompts on the 5th-generation tensor cores.
+//
+// o_i = sum_j p_ij v_j, p = softmax over the visible keys of scale * q_i k_j, one pass over the keys with a running maximum and
+// sum.  Bound by the tensor pipe and, as closely, by the exponentials: a 128 x 128 tile of scores costs 512 cycles of products
+// each for S = Q K^T and O += P V at head size 128, and 128 * 128 / 16 = 1024 cycles of the SM's exp2 unit.
+//
+// The query heads of one key-value head are rows of one tile: 128 / g tokens x g heads (g = heads / kv_heads), so a group reads
+// its keys and values once, and a tile spans few tokens, which keeps what is computed above the diagonal small.  A CTA works
+// on two such tiles (256 rows) against the same key blocks of 128, so that one tile's softmax runs under the other's products.
+// Persistent CTAs, one per SM, walk a list of (tile pair, kv head), the longest first.  Roles:
+//   warp 0     loads Q (both tiles) and K blocks by TMA            warp 3   loads V blocks
+//   warp 1     issues every tcgen05.mma: S of both tiles into tensor memory, then per block P V into the output accumulator
+//              (P is read from tensor memory, where it overwrites its own S)
+//   warp 2     makes V blocks that some row must not see in part safe (below)
+//   warps 4-7, 8-11   softmax of the first and second tile, a row per thread; rescale and write the output
+// The output accumulator is rescaled only when a row's maximum has grown by more than 2^6; until then weights are taken against
+// the older maximum, which stays inside fp16's range.
+// A masked weight is 0, but 0 x NaN and 0 x infinity are not.  So the blocks that reach over the diagonal or the sequence's
+// end are looked through before their product: their non-finite values become 0 in shared memory, and if there were any,
+// the rows that do see them get them added at the end from global memory (a weight is positive, so infinities keep their sign).
 #include "moe_attn.cuh"
+#include "moe_tc.cuh"
 
 namespace {
 
-struct AttnArgs {
-    const __half *q, *k, *v;
-    const uint32_t *cu_q, *cu_k;
-    __half *o;
-    moe_pc_attn_t pc;
-    uint32_t group;
-};
+using namespace moe_tc;
+
+constexpr uint32_t AT_THREADS = 384, TILE_ROWS = 128, BLOCK_KEYS = 128;
+constexpr uint32_t HALF_BYTES = 128 * 128;       // 128 rows of 64 columns, one TMA box
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float GROW = 6.0f;                     // log2 of how far weights may pass the reference before a rescale
+constexpr float SHIFT = 8.0f;                    // weights are at most 2^(GROW + SHIFT) = 2^14; fp16 then goes down to 2^-32 of the reference
+constexpr uint32_t FLAGS = 8;                    // items that may be between their V check and their epilogue
 
 template <uint32_t HD>
-__global__ void __launch_bounds__(128) moe_attn_kernel(AttnArgs a) {
-    __shared__ float qs[4][HD];
-    moe_pdl_begin();
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint64_t total = (uint64_t)min(a.cu_q[a.pc.seqs], a.pc.rows_q) * a.pc.heads;
-    for (uint64_t w = (uint64_t)blockIdx.x * 4u + warp; w < total; w += (uint64_t)gridDim.x * 4u) {
-        const uint32_t row = (uint32_t)(w / a.pc.heads), head = (uint32_t)(w % a.pc.heads), kh = head / a.group;
-        uint32_t lo = 0, hi = a.pc.seqs;
-        while (hi - lo > 1u) {
-            const uint32_t mid = (lo + hi) / 2u;
-            if (a.cu_q[mid] <= row) lo = mid;
-            else hi = mid;
+struct Cfg {
+    static constexpr uint32_t HALVES = HD / 64;
+    static constexpr uint32_t TILE_BYTES = HALVES * HALF_BYTES;      // Q tile, K block or V block
+    static constexpr uint32_t STAGES = HD == 128 ? 5 : 8;
+    static constexpr uint32_t SMEM = (2 + STAGES) * TILE_BYTES;
+};
+
+template <uint32_t ST>
+struct __align__(8) AttnBars {
+    uint64_t kv_full[ST], kv_empty[ST];
+    uint64_t v_landed[ST];   // masked V blocks: loaded; warp 2 then arrives at kv_full
+    uint64_t q_full, q_empty;
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint64_t drain;          // unwinding: all products issued have retired
+    uint32_t tmem_base, abort;
+    uint32_t found[FLAGS];   // the item's masked V blocks held something that is not finite
+};
+
+// A pair of tiles of one sequence: `left` queries from row q_row on, the sequence's keys from row k_row on.
+struct Pair {
+    uint32_t q_row, left, k_row, lk;
+};
+
+struct AttnArgs {
+    const uint32_t *cu_q, *cu_k;
+    const __half *v;
+    __half *o;
+    const uint4 *plan;       // NULL: one sequence, its pairs from the last to the first
+    const uint32_t *pairs;   // number of entries of plan
+    uint32_t rows_q, rows_k, kv_heads, group, tile_tokens;
+    uint32_t kv_stride, o_stride;
+    float scale;
+    uint32_t *status;
+    uint64_t wait_ns;
+};
+
+// Rows a .. b - 1 of a table of `rows`, whatever the caller's offsets are.
+__device__ __forceinline__ uint32_t span(uint32_t a, uint32_t b, uint32_t rows) {
+    return a <= b && b <= rows ? b - a : 0u;
+}
+
+// What a CTA has to do, in turn: round r takes item r * G + c, odd rounds from the other end, so that with falling costs every
+// CTA gets about the same.
+struct Items {
+    uint32_t count, round;
+    Pair one;
+    uint32_t one_pairs;
+
+    __device__ __forceinline__ void begin(const AttnArgs &a) {
+        round = 0;
+        if (a.plan == nullptr) {
+            one.q_row = a.cu_q[0];
+            one.left = span(a.cu_q[0], a.cu_q[1], a.rows_q);
+            one.k_row = a.cu_k[0];
+            one.lk = span(a.cu_k[0], a.cu_k[1], a.rows_k);
+            one_pairs = (one.left + 2u * a.tile_tokens - 1u) / (2u * a.tile_tokens);
+            count = one_pairs * a.kv_heads;
+        } else {
+            count = *a.pairs * a.kv_heads;
         }
-        const int64_t k0 = a.cu_k[lo], k1 = min(a.cu_k[lo + 1u], a.pc.rows_k), lk = max(k1 - k0, (int64_t)0);
-        const int64_t seen = (int64_t)row - a.cu_q[lo + 1u] + lk + 1;
-        for (uint32_t d = lane; d < HD; d += 32u) qs[warp][d] = __half2float(a.q[(size_t)row * a.pc.q_stride + head * HD + d]) * a.pc.scale;
-        __syncwarp();
-        float m = -INFINITY, l = 0.0f, o[HD / 32u] = {};
-        for (int64_t j0 = 0; j0 < seen; j0 += 32) {
-            const int64_t j = j0 + lane;
-            float s = -INFINITY;
-            if (j < seen) {
-                const __half *kr = a.k + (size_t)(k0 + j) * a.pc.kv_stride + kh * HD;
-                s = 0.0f;
-                for (uint32_t d = 0; d < HD; d += 1) s += qs[warp][d] * __half2float(kr[d]);
-            }
-            float t = s;
-            for (uint32_t x = 16; x != 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, x));
-            t = fmaxf(m, t);
-            const float keep = m == t ? 1.0f : expf(m - t), p = t == -INFINITY ? 0.0f : expf(s - t);
-            float sum = p;
-            for (uint32_t x = 16; x != 0; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
-            l = l * keep + sum;
-            m = t;
-            for (uint32_t i = 0; i < HD / 32u; i += 1) o[i] *= keep;
-            for (uint32_t x = 0; x < 32u && j0 + x < seen; x += 1) {
-                const float pj = __shfl_sync(~0u, p, x);
-                const __half *vr = a.v + (size_t)(k0 + j0 + x) * a.pc.kv_stride + kh * HD;
-                for (uint32_t i = 0; i < HD / 32u; i += 1) o[i] += pj * __half2float(vr[i * 32u + lane]);
-            }
-        }
-        for (uint32_t i = 0; i < HD / 32u; i += 1) {
-            a.o[(size_t)row * a.pc.o_stride + head * HD + i * 32u + lane] = __float2half(l == 0.0f ? 0.0f : o[i] / l);
-        }
-        __syncwarp();
     }
+    __device__ __forceinline__ bool next(const AttnArgs &a, Pair &p, uint32_t &head) {
+        const uint32_t at = round * gridDim.x + ((round & 1u) != 0 ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
+        if (at >= count) return false;   // a round that is too short for this CTA is the last one
+        round += 1;
+        take(a, at, p, head);
+        return true;
+    }
+    __device__ __forceinline__ void take(const AttnArgs &a, uint32_t at, Pair &p, uint32_t &head) {
+        const uint32_t i = at / a.kv_heads;
+        head = at - i * a.kv_heads;
+        if (a.plan == nullptr) {
+            const uint32_t q0 = (one_pairs - 1u - i) * 2u * a.tile_tokens;
+            p.q_row = one.q_row + q0;
+            p.left = one.left - q0;
+            p.k_row = one.k_row;
+            p.lk = one.lk;
+        } else {
+            const uint4 e = a.plan[i];
+            p.q_row = e.x;
+            p.left = e.y;
+            p.k_row = e.z;
+            p.lk = e.w;
+        }
+    }
+};
+
+// Visible keys of the query `i` behind the pair's first one (may be negative).
+__device__ __forceinline__ int32_t visible(const Pair &p, uint32_t i) { return (int32_t)p.lk - (int32_t)p.left + 1 + (int32_t)i; }
+
+struct Blocks {
+    uint32_t tile[2];   // key blocks that the tile's last query sees; 0: the tile has no query, or its queries no key
+    bool has_b;
+    uint32_t n;
+    int32_t masked_from;  // blocks from here on are masked for some row
+};
+__device__ __forceinline__ Blocks blocks_of(const Pair &p, uint32_t tile_tokens) {
+    Blocks b;
+    b.has_b = p.left > tile_tokens;
+    const int32_t va = visible(p, min(p.left, tile_tokens) - 1u), vb = b.has_b ? visible(p, min(p.left, 2u * tile_tokens) - 1u) : 0;
+    b.tile[0] = va > 0 ? ((uint32_t)va + BLOCK_KEYS - 1u) / BLOCK_KEYS : 0u;
+    b.tile[1] = vb > 0 ? ((uint32_t)vb + BLOCK_KEYS - 1u) / BLOCK_KEYS : 0u;
+    b.n = max(b.tile[0], b.tile[1]);
+    const int32_t first = visible(p, 0);
+    b.masked_from = first > 0 ? first / (int32_t)BLOCK_KEYS : 0;
+    return b;
+}
+
+// V as the second operand of P V: [keys][columns] with the columns contiguous ("MN-major"), 128-byte swizzle: 64-column
+// groups HALF_BYTES apart, groups of 8 keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3ffffu) >> 4) | ((uint64_t)(HALF_BYTES >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D[tmem] (+)= A[tmem] * B
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+        :
+        : "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t c0, int32_t c1, int32_t c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        :
+        : "r"(dst), "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+        "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// mbar_wait without a call, so that the registers of a softmax thread need not follow a calling convention.
+__device__ __forceinline__ bool wait_here(uint32_t bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t site, uint64_t wait_ns) {
+    uint32_t spins = 0;
+    uint64_t t0 = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        spins += 1;
+        if ((spins & 0xffu) != 0) continue;
+        if (*abort != 0) return false;
+        const uint64_t now = globaltimer_ns();
+        if (t0 == 0) {
+            t0 = now;
+        } else if (now - t0 > wait_ns) {
+            *abort = 1;
+            atomicCAS(status, 0u, (uint32_t)MOE_ERR_TIMEOUT | (site << 8));
+            return false;
+        }
+    }
+    return true;
+}
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(AT_THREADS, 1)
+moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                AttnArgs a) {
+    using C = Cfg<HD>;
+    constexpr uint32_t ST = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    AttnBars<ST> *bars = reinterpret_cast<AttnBars<ST> *>(smem + C::SMEM);
+    const uint32_t q_smem = smem_u32(smem), ring = q_smem + 2u * C::TILE_BYTES;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    volatile uint32_t *abort = &bars->abort;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < ST; i += 1) {
+            mbar_init(smem_u32(&bars->kv_full[i]), 1);
+            mbar_init(smem_u32(&bars->kv_empty[i]), 1);
+            mbar_init(smem_u32(&bars->v_landed[i]), 1);
+        }
+        mbar_init(smem_u32(&bars->q_full), 1);
+        mbar_init(smem_u32(&bars->q_empty), 1);
+        mbar_init(smem_u32(&bars->drain), 1);
+        for (uint32_t i = 0; i < 2; i += 1) {
+            mbar_init(smem_u32(&bars->s_full[i]), 1);
+            mbar_init(smem_u32(&bars->p_full[i]), TILE_ROWS);
+            mbar_init(smem_u32(&bars->o_full[i]), 1);
+            mbar_init(smem_u32(&bars->o_empty[i]), TILE_ROWS);
+        }
+        bars->abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bars->tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;   // S of the two tiles at 0 and 128, O at 256 and 256 + HD
+
+    moe_pdl_begin();
+
+    Items items;
+    items.begin(a);
+    Pair p;
+    uint32_t head;
+#define AT_WAIT(bar, parity, site) wait_here(smem_u32(bar), (parity), abort, a.status, (site), a.wait_ns)
+
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.plan == nullptr &&
+        (a.cu_q[0] > a.cu_q[1] || a.cu_q[1] > a.rows_q || a.cu_k[0] > a.cu_k[1] || a.cu_k[1] > a.rows_k)) {
+        moe_deny(a.status, MOE_SITE_ROWS);
+    }
+    // 384 threads start with 168 registers: the softmax keeps a whole row of scores in them, the other warps need few
+    if (warp < 4u) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 0 || warp == 3) {
+            // ---------------- loads: ring places K(n-1), V(n-1), K(n-2), V(n-2), ... of each item in turn ----------------
+            if (lane == 0) {
+                const bool is_v = warp == 3;
+                uint32_t at = is_v ? 1u : 0u, q_phase = 1, issued = 0, parity = 0, masked = 0, landed = 0;
+                uint32_t q_bytes = 0, q_loads = 0;
+                bool ok = true;
+                while (ok && items.next(a, p, head)) {
+                    const Blocks b = blocks_of(p, a.tile_tokens);
+                    if (b.n == 0) continue;
+                    if (!is_v) {
+                        if (!AT_WAIT(&bars->q_empty, q_phase, 31)) break;
+                        q_phase ^= 1u;
+                        q_bytes = a.group * a.tile_tokens * 128u * C::HALVES * (b.has_b ? 2u : 1u);
+                        mbar_expect_tx(smem_u32(&bars->q_full), q_bytes);
+                        for (uint32_t t = 0; t < (b.has_b ? 2u : 1u); t += 1) {
+                            for (uint32_t h = 0; h < C::HALVES; h += 1) {
+                                tma_load_3d(q_smem + t * C::TILE_BYTES + h * HALF_BYTES, &tm_q, smem_u32(&bars->q_full), (int32_t)(h * 64u),
+                                            (int32_t)(head * a.group), (int32_t)(p.q_row + t * a.tile_tokens));
+                            }
+                        }
+                        q_loads += 1;
+                    }
+                    for (uint32_t j = b.n; j-- > 0;) {
+                        const uint32_t s = at % ST, ph = (at / ST) & 1u;
+                        if (!AT_WAIT(&bars->kv_empty[s], ph ^ 1u, 32)) {
+                            ok = false;
+                            break;
+                        }
+                        const bool m = is_v && (int32_t)j >= b.masked_from;
+                        const uint32_t full = smem_u32(m ? &bars->v_landed[s] : &bars->kv_full[s]);
+                        mbar_expect_tx(full, C::TILE_BYTES);
+                        for (uint32_t h = 0; h < C::HALVES; h += 1) {
+                            tma_load_3d(ring + s * C::TILE_BYTES + h * HALF_BYTES, is_v ? &tm_v : &tm_k, full, (int32_t)(h * 64u), (int32_t)head,
+                                        (int32_t)(p.k_row + j * BLOCK_KEYS));
+                        }
+                        issued |= 1u << s;
+                        parity = (parity & ~(1u << s)) | (ph << s);
+                        masked = (masked & ~(1u << s)) | ((m ? 1u : 0u) << s);
+                        landed ^= (m ? 1u : 0u) << s;   // the next masked use's parity
+                        at += 2u;
+                    }
+                }
+                if (*abort != 0) {
+                    // unwinding: give copies already issued a bounded time to land
+                    for (uint32_t s = 0; s < ST; s += 1) {
+                        for (uint32_t spin = 0; (issued >> s & 1u) != 0 && spin < (1u << 16); spin += 1) {
+                            if ((masked >> s & 1u) != 0) {
+                                if (mbar_try_wait(smem_u32(&bars->v_landed[s]), ~landed >> s & 1u)) break;
+                            } else if (mbar_try_wait(smem_u32(&bars->kv_full[s]), parity >> s & 1u)) {
+                                break;
+                            }
+                        }
+                    }
+                    for (uint32_t spin = 0; q_loads != 0 && spin < (1u << 16); spin += 1) {
+                        if (mbar_try_wait(smem_u32(&bars->q_full), (q_loads - 1u) & 1u)) break;
+                    }
+                }
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ---------------- MMA issue: the whole warp runs the loop, one elected lane issues ----------------
+            uint32_t at = 0, q_phase = 0, p_phase = 0, o_phase = 3;
+            bool ok = true;
+            const uint32_t idesc_s = umma_idesc(128, BLOCK_KEYS), idesc_o = umma_idesc(128, HD) | (1u << 16);  // V: MN-major
+            auto scores = [&](uint32_t t, uint32_t slot) {
+                if (elect_one()) {
+                    const uint64_t qd = umma_desc(q_smem + t * C::TILE_BYTES), kd = umma_desc(ring + slot * C::TILE_BYTES);
+#pragma unroll
+                    for (uint32_t k = 0; k < HD / 16u; k += 1) {
+                        const uint64_t off = (uint64_t)((k / 4u) * (HALF_BYTES >> 4) + (k % 4u) * 2u);
+                        umma_f16(tmem + t * 128u, qd + off, kd + off, idesc_s, k != 0 ? 1u : 0u);
+                    }
+                    umma_commit(smem_u32(&bars->s_full[t]));
+                }
+                __syncwarp();
+            };
+            while (ok && items.next(a, p, head)) {
+                const Blocks b = blocks_of(p, a.tile_tokens);
+                if (b.n == 0) continue;
+                if (!AT_WAIT(&bars->q_full, q_phase, 33)) break;
+                q_phase ^= 1u;
+                uint32_t ks = at % ST;
+                if (!AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34)) break;
+                __syncwarp();
+                tc_fence_after();
+                for (uint32_t t = 0; t < 2; t += 1) {
+                    if (b.n == b.tile[t]) scores(t, ks);
+                }
+                if (elect_one()) {
+                    umma_commit(smem_u32(&bars->kv_empty[ks]));
+                    if (b.n == 1u) umma_commit(smem_u32(&bars->q_empty));
+                }
+                __syncwarp();
+                for (uint32_t j = b.n; j-- > 0 && ok;) {
+                    const uint32_t vi = at + 1u, vs = vi % ST;
+                    ok = AT_WAIT(&bars->kv_full[vs], (vi / ST) & 1u, 35);
+                    at += 2u;
+                    ks = at % ST;
+                    if (ok && j != 0) ok = AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34);
+                    for (uint32_t t = 0; t < 2u && ok; t += 1) {
+                        if (j < b.tile[t]) {
+                            const bool first = j + 1u == b.tile[t];
+                            if (first) {
+                                ok = AT_WAIT(&bars->o_empty[t], o_phase >> t & 1u, 37);
+                                o_phase ^= 1u << t;
+                            }
+                            ok = ok && AT_WAIT(&bars->p_full[t], p_phase >> t & 1u, 38);
+                            p_phase ^= 1u << t;
+                            if (!ok) break;
+                            __syncwarp();
+                            tc_fence_after();
+                            if (elect_one()) {
+                                const uint64_t vd = v_desc(ring + vs * C::TILE_BYTES);
+#pragma unroll
+                                for (uint32_t k = 0; k < BLOCK_KEYS / 16u; k += 1) {
+                                    umma_f16_ts(tmem + 256u + t * HD, tmem + t * 128u + k * 8u, vd + k * 128u, idesc_o, first && k == 0 ? 0u : 1u);
+                                }
+                                if (j == 0) umma_commit(smem_u32(&bars->o_full[t]));
+                            }
+                            __syncwarp();
+                        }
+                        if (j != 0 && j - 1u < b.tile[t]) {
+                            __syncwarp();
+                            tc_fence_after();
+                            scores(t, ks);
+                        }
+                    }
+                    if (!ok) break;
+                    if (elect_one()) {
+                        umma_commit(smem_u32(&bars->kv_empty[vs]));
+                        if (j != 0) umma_commit(smem_u32(&bars->kv_empty[ks]));
+                        if (j == 1u) umma_commit(smem_u32(&bars->q_empty));
+                    }
+                    __syncwarp();
+                }
+            }
+            __syncwarp();
+            if (*abort != 0) {
+                // unwinding: a bounded time for the products already issued
+                if (elect_one()) umma_commit(smem_u32(&bars->drain));
+                __syncwarp();
+                for (uint32_t spin = 0; spin < (1u << 16); spin += 1) {
+                    if (mbar_try_wait(smem_u32(&bars->drain), 0)) break;
+                }
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // ---------------- V blocks that reach over the diagonal or the sequence's end ----------------
+            uint32_t at = 0, n_item = 0, landed = 0;
+            bool ok = true;
+            while (ok && items.next(a, p, head)) {
+                const Blocks b = blocks_of(p, a.tile_tokens);
+                if (b.n == 0) continue;
+                volatile uint32_t *found = &bars->found[n_item % FLAGS];
+                if (lane == 0) *found = 0;
+                __syncwarp();
+                for (uint32_t j = b.n; j-- > 0 && (int32_t)j >= b.masked_from;) {
+                    const uint32_t vi = at + 2u * (b.n - 1u - j) + 1u, vs = vi % ST;
+                    if (!AT_WAIT(&bars->v_landed[vs], landed >> vs & 1u, 39)) {
+                        ok = false;
+                        break;
+                    }
+                    landed ^= 1u << vs;
+                    __syncwarp();
+                    uint8_t *block = smem + (2u + vs) * C::TILE_BYTES;
+                    uint32_t most = 0;   // the largest exponent and mantissa of either half
+#pragma unroll 8
+                    for (uint32_t i = lane; i < C::TILE_BYTES / 16u; i += 32u) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(block + i * 16u);
+                        most = __vmaxu2(__vmaxu2(__vmaxu2(most, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, w.z & 0x7fff7fffu)), w.w & 0x7fff7fffu);
+                    }
+                    if (__any_sync(0xffffffffu, (most & 0xffffu) >= 0x7c00u || (most >> 16) >= 0x7c00u)) {
+                        for (uint32_t i = lane; i < C::TILE_BYTES / 4u; i += 32u) {
+                            uint32_t *w = reinterpret_cast<uint32_t *>(block + i * 4u);
+                            uint32_t x = *w;
+                            if ((x & 0x7c00u) == 0x7c00u) x &= 0xffff0000u;
+                            if ((x & 0x7c000000u) == 0x7c000000u) x &= 0xffffu;
+                            *w = x;
+                        }
+                        if (lane == 0) *found = 1;
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&bars->kv_full[vs]));
+                }
+                at += 2u * b.n;
+                n_item += 1;
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ---------------- softmax and output: a row per thread ----------------
+        const uint32_t t = (warp - 4u) >> 2, row = (warp & 3u) * 32u + lane;
+        const uint32_t my_token = row / a.group, my_head = row - my_token * a.group;
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16;
+        const uint32_t s_at = tmem + t * 128u + lanes, o_at = tmem + 256u + t * HD + lanes;
+        const float to_log2 = a.scale * LOG2E;
+        uint32_t s_phase = 0, o_phase = 0, n_item = 0;
+        bool ok = true;
+        while (ok && items.next(a, p, head)) {
+            const Blocks b = blocks_of(p, a.tile_tokens);
+            const uint32_t token = t * a.tile_tokens + my_token;   // behind the pair's first
+            const bool mine = my_token < a.tile_tokens && token < p.left;
+            __half *out = a.o + (size_t)(p.q_row + token) * a.o_stride + (size_t)(head * a.group + my_head) * HD;
+            const uint32_t n = b.tile[t], flag = n_item % FLAGS;
+            if (b.n != 0) n_item += 1;
+            if (n == 0) {   // no query, or none that sees a key
+                if (mine) {
+#pragma unroll
+                    for (uint32_t i = 0; i < HD; i += 8) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
+                }
+                continue;
+            }
+            const int32_t vis = visible(p, token);
+            const int32_t tile_first = visible(p, t * a.tile_tokens);
+            float top = -INFINITY, sum = 0.0f;   // top: the reference that weights are taken against, in score units
+            for (uint32_t j = n; j-- > 0;) {
+                if (!AT_WAIT(&bars->s_full[t], s_phase, 40)) {
+                    ok = false;
+                    break;
+                }
+                s_phase ^= 1u;
+                __syncwarp();
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i += 1) tmem_ld32(s_at + i * 32u, s[i]);
+                tmem_ld_wait();
+                if ((int32_t)((j + 1u) * BLOCK_KEYS) > tile_first) {
+                    const int32_t seen = vis - (int32_t)(j * BLOCK_KEYS);   // columns below it are visible
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i += 1) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 32; e += 1) {
+                            if ((int32_t)(i * 32u + e) >= seen) s[i][e] = 0xff800000u;
+                        }
+                    }
+                }
+                float m[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i += 1) {
+                    m[i] = __uint_as_float(s[i][0]);
+#pragma unroll
+                    for (uint32_t e = 1; e < 32; e += 1) m[i] = fmaxf(m[i], __uint_as_float(s[i][e]));
+                }
+                const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                const bool grows = (now - top) * to_log2 > GROW;   // also from -infinity; not from there to there
+                if (j + 1u == n) {
+                    top = now;
+                } else if (__any_sync(0xffffffffu, grows)) {
+                    // P V of the blocks before has completed: this S was issued behind it
+                    const float f = grows ? exp2_fast((top - now) * to_log2) : 1.0f;
+                    if (grows) top = now;
+                    sum *= f;
+#pragma unroll
+                    for (uint32_t i = 0; i < HD / 32u; i += 1) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + i * 32u, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (uint32_t e = 0; e < 32; e += 1) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(o_at + i * 32u, o);
+                    }
+                }
+                const float base = top == -INFINITY ? 0.0f : SHIFT - top * to_log2;
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i += 1) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; e += 1) {
+                        const float x = exp2_fast(fmaf(__uint_as_float(s[i][2 * e]), to_log2, base));
+                        const float y = exp2_fast(fmaf(__uint_as_float(s[i][2 * e + 1]), to_log2, base));
+                        part[e & 3u] += x + y;
+                        // weights round to fp16 for the product (11 bits, as many as the output has); their sum does not
+                        w[e] = pack_h2(x, y);
+                    }
+                    tmem_st16(s_at + i * 16u, w);
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars->p_full[t]));
+            }
+            if (!ok || !AT_WAIT(&bars->o_full[t], o_phase, 41)) break;
+            o_phase ^= 1u;
+            __syncwarp();
+            tc_fence_after();
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const bool extra = *(volatile uint32_t *)&bars->found[flag] != 0;
+            for (uint32_t i = 0; i < HD / 32u; i += 1) {
+                uint32_t o[32];
+                tmem_ld32(o_at + i * 32u, o);
+                tmem_ld_wait();
+                if (mine) {
+                    float y[32];
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; e += 1) y[e] = sum == 0.0f ? 0.0f : __uint_as_float(o[e]) * f;
+                    if (extra) {
+                        for (int32_t key = b.masked_from * (int32_t)BLOCK_KEYS; key < vis; key += 1) {
+                            const __half *v = a.v + (size_t)(p.k_row + (uint32_t)key) * a.kv_stride + (size_t)head * HD + i * 32u;
+#pragma unroll
+                            for (uint32_t e = 0; e < 32; e += 1) {
+                                const float x = __half2float(v[e]);
+                                if (!isfinite(x)) y[e] += x;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; e += 8) {
+                        *reinterpret_cast<uint4 *>(out + i * 32u + e) =
+                            make_uint4(pack_h2(y[e], y[e + 1]), pack_h2(y[e + 2], y[e + 3]), pack_h2(y[e + 4], y[e + 5]), pack_h2(y[e + 6], y[e + 7]));
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            mbar_arrive(smem_u32(&bars->o_empty[t]));
+        }
+    }
+#undef AT_WAIT
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// The list of tile pairs, those with the most key blocks first (counting sort over 1024 classes of cost; the order within a
+// class does not matter to any result).
+constexpr uint32_t PLAN_THREADS = 1024, CLASSES = 1024;
+__global__ void __launch_bounds__(PLAN_THREADS) moe_attn_plan_kernel(AttnArgs a, uint32_t seqs, uint4 *plan, uint32_t *pairs) {
+    __shared__ uint32_t place[CLASSES];
+    __shared__ uint32_t warp_sum[32];
+    __shared__ uint32_t most;
+    moe_pdl_begin();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, step = 2u * a.tile_tokens;
+    place[threadIdx.x] = 0;
+    if (threadIdx.x == 0) most = 1;
+    __syncthreads();
+    uint32_t longest = 0;
+    for (uint32_t s = threadIdx.x; s < seqs; s += PLAN_THREADS) {
+        if (a.cu_q[s] > a.cu_q[s + 1u] || a.cu_q[s + 1u] > a.rows_q || a.cu_k[s] > a.cu_k[s + 1u] || a.cu_k[s + 1u] > a.rows_k)
+            moe_deny(a.status, MOE_SITE_ROWS);
+        longest = max(longest, span(a.cu_k[s], a.cu_k[s + 1u], a.rows_k));
+    }
+    atomicMax(&most, longest);
+    __syncthreads();
+    const uint32_t per = (most / BLOCK_KEYS + 1u) / CLASSES + 1u;   // key blocks of one class
+    for (uint32_t pass = 0; pass < 2; pass += 1) {
+        for (uint32_t s = warp; s < seqs; s += PLAN_THREADS / 32u) {
+            Pair p;
+            const uint32_t q0 = a.cu_q[s], lq = span(q0, a.cu_q[s + 1u], a.rows_q);
+            p.k_row = a.cu_k[s];
+            p.lk = span(p.k_row, a.cu_k[s + 1u], a.rows_k);
+            for (uint32_t i = lane * step; i < lq; i += 32u * step) {
+                p.q_row = q0 + i;
+                p.left = lq - i;
+                const uint32_t n = min(CLASSES - 1u, blocks_of(p, a.tile_tokens).n / per), cls = CLASSES - 1u - n;
+                const uint32_t at = atomicAdd(&place[cls], 1u);
+                if (pass != 0) plan[at] = make_uint4(p.q_row, p.left, p.k_row, p.lk);
+            }
+        }
+        __syncthreads();
+        if (pass != 0) break;
+        const uint32_t mine = place[threadIdx.x];
+        uint32_t incl = mine;
+#pragma unroll
+        for (uint32_t o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        uint32_t before = 0;
+        for (uint32_t w = 0; w < warp; w += 1) before += warp_sum[w];
+        place[threadIdx.x] = before + incl - mine;
+        if (threadIdx.x == PLAN_THREADS - 1u) *pairs = before + incl;
+        __syncthreads();
+    }
+}
+
+template <uint32_t HD>
+void attn_launch(moe_cuda_ctx *c, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, uint32_t grid, uint32_t slot) {
+    constexpr uint32_t smem = Cfg<HD>::SMEM + sizeof(AttnBars<Cfg<HD>::STAGES>) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of one SM");
+    if (!c->attn_attr_set[slot]) {
+        MOE_CUDA_TRY(c, cudaFuncSetAttribute(moe_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        c->attn_attr_set[slot] = true;
+    }
+    moe_run(c, moe_attn_kernel<HD>, grid, AT_THREADS, smem, tq, tk, tv, a);
+    MOE_LAUNCHED(c);
 }
 
 }  // namespace
@@ -68,10 +670,47 @@ extern "C" void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k1
     const char *why = moe_attn_refusal(q16, k16, v16, cu_q, cu_k, o16, pc);
     MOE_REQUIRE(c, why == NULL, "%s", why);
     if (pc.rows_q == 0 || pc.seqs == 0) return;
+    AttnArgs a;
+    a.cu_q = cu_q;
+    a.cu_k = cu_k;
+    a.v = (const __half *)v16;
+    a.o = (__half *)o16;
+    a.plan = NULL;
+    a.pairs = NULL;
+    a.rows_q = pc.rows_q;
+    a.rows_k = pc.rows_k;
+    a.kv_heads = pc.kv_heads;
+    a.group = pc.heads / pc.kv_heads;
+    a.tile_tokens = TILE_ROWS / a.group;
+    a.kv_stride = pc.kv_stride;
+    a.o_stride = pc.o_stride;
+    a.scale = pc.scale;
+    a.status = c->dev_status_dev;
+    a.wait_ns = c->wait_ns;
+    const uint64_t pairs = (uint64_t)pc.rows_q / (2u * a.tile_tokens) + pc.seqs;   // at most
+    MOE_REQUIRE(c, pairs * pc.kv_heads < (1ull << 31), "attn: too many tiles");
+    CUtensorMap tq, tk, tv;
+    if (!moe_tmap_heads_f16(c, &tq, q16, pc.rows_q, pc.heads, pc.hd, pc.q_stride, a.group, a.tile_tokens)) return;
+    if (pc.rows_k == 0) {
+        tk = tv = tq;   // never loaded from
+    } else if (!moe_tmap_heads_f16(c, &tk, k16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS) ||
+               !moe_tmap_heads_f16(c, &tv, v16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS)) {
+        return;
+    }
     moe_on_device on(c);
-    AttnArgs a = {(const __half *)q16, (const __half *)k16, (const __half *)v16, cu_q, cu_k, (__half *)o16, pc, pc.heads / pc.kv_heads};
-    const uint32_t grid = (uint32_t)c->sm_count * 16u;
-    if (pc.hd == 128u) moe_run(c, moe_attn_kernel<128>, grid, 128, 0, a);
-    else moe_run(c, moe_attn_kernel<64>, grid, 128, 0, a);
-    MOE_LAUNCHED(c);
+    if (pc.seqs > 1u) {
+        const size_t need = 256 + (size_t)pairs * sizeof(uint4);
+        if (need > c->work_bytes) {
+            moe_fail(c, MOE_ERR_NOMEM, "attn: %zu bytes of work area, the context has %zu", need, c->work_bytes);
+            return;
+        }
+        a.pairs = (const uint32_t *)c->work;
+        a.plan = (const uint4 *)((uint8_t *)c->work + 256);
+        moe_run(c, moe_attn_plan_kernel, 1, PLAN_THREADS, 0, a, pc.seqs, (uint4 *)a.plan, (uint32_t *)a.pairs);
+        MOE_LAUNCHED(c);
+    }
+    const uint64_t items = pairs * pc.kv_heads;
+    const uint32_t grid = items < (uint64_t)c->sm_count ? (uint32_t)items : (uint32_t)c->sm_count;
+    if (pc.hd == 128u) attn_launch<128>(c, tq, tk, tv, a, grid, 0);
+    else attn_launch<64>(c, tq, tk, tv, a, grid, 1);
 }

@@ -395,3 +395,12 @@ bool moe_tmap_tokens_f16(moe_cuda_ctx *c, moe_xmaps *out, const void *ptr, uint6
     memcpy(&t->maps, out, sizeof(*out));
     return true;
 }
+
+// Heads side by side in rows of `stride`: boxes of 64 columns, `box_heads` heads, `box_rows` rows, in shared memory row by
+// row and within a row head by head.
+bool moe_tmap_heads_f16(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint32_t rows, uint32_t heads, uint32_t hd, uint32_t stride,
+                        uint32_t box_heads, uint32_t box_rows) {
+    const cuuint64_t dims[3] = {hd, heads, rows}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_rows};
+    return moe_encode(c, out, 3, ptr, dims, strides, box);
+}

@@ -378,3 +378,27 @@ def test_attn_many_sequences(on):
 
 def test_attn_long(on):
     _attn(on, _gen(5), [5000], [6001], 8, 2, 128)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,lq,lk", [(16, 2, [384] * 32, [384] * 32), (12, 4, [700] * 9, [1100] * 9), (1, 1, [20000], [20000]),
+                                                  (16, 1, [900, 3, 1500], [900, 3, 1500])])
+def test_attn_several_items_to_every_sm_and_call_after_call(on, hd, heads, kv_heads, lq, lk):
+    """More tile pairs than SMs, of one key block and of many, and calls one behind the other without a wait between."""
+    g = _gen(heads)
+    nq, nk = sum(lq), sum(lk)
+    q, k, v = _f16(g, nq, heads, hd), _f16(g, nk, kv_heads, hd), _f16(g, nk, kv_heads, hd)
+    cq, ck = _starts(lq), _starts(lk)
+    outs = [torch.full_like(q, 7.0) for _ in range(4)]
+    for out in outs:
+        on.attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), cq.data_ptr(), ck.data_ptr(), out.data_ptr(), len(lq), nq, nk, heads, kv_heads, hd)
+    on.flush()
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])
+    a = b = 0
+    for m, n in zip(lq, lk):
+        for lo in range(0, m, 2500):   # query rows in pieces
+            hi = min(m, lo + 2500)
+            o, mass, size = R.attention(q[a + lo:a + hi].double(), k[b:b + n].double(), v[b:b + n].double(), hd ** -0.5, n - m + lo)
+            R.check(outs[0][a + lo:a + hi], o, mass, size, hd, n)
+        a, b = a + m, b + n
