@@ -231,7 +231,7 @@ void moe_cuda_rope(moe_cuda_ctx_t *c, const float *x, const uint32_t *pos, void 
  * page g is slot g * page + p.  MOE_KV_E4M3 holds 8-bit floats (e4m3) and, for
  * every slot and kv head, one positive scale each for keys and values
  * ([pages][kv_heads][page] fp32): value = code * scale.  hd 64 or 128; page a power of two
- * from 16 to 256; fewer than 2^32 - 1 slots. */
+ * from 16 to 256; slots * kv_heads below 2^31. */
 typedef struct moe_cuda_kv_t {
     void *k, *v;
     float *k_scale, *v_scale; /* MOE_KV_E4M3 only */

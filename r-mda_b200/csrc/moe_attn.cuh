@@ -35,3 +35,10 @@ __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t codes) {
     asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}\n" : "=r"(h2) : "r"(codes));
     return h2;
 }
+
+// Four e4m3 codes as two pairs of fp16 values.
+__device__ __forceinline__ void e4m3x4_to_h2(uint32_t codes, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(codes));
+}

@@ -33,8 +33,9 @@ static inline const char *moe_kv_refusal(const moe_cuda_kv_t *kv) {
     if (kv->type != MOE_KV_F16 && kv->type != MOE_KV_E4M3) return "cache: type is MOE_KV_F16 or MOE_KV_E4M3";
     if (kv->hd != 64u && kv->hd != 128u) return "cache: hd is 64 or 128";
     if (kv->page < 16u || kv->page > 256u || (kv->page & (kv->page - 1u)) != 0) return "cache: page is a power of two from 16 to 256";
-    if (kv->pages == 0 || (uint64_t)kv->pages * kv->page >= 0xffffffffull) return "cache: 1 to 2^32 - 2 slots";
+    if (kv->pages == 0 || (uint64_t)kv->pages * kv->page >= (1ull << 31)) return "cache: 1 to 2^31 - 1 slots";
     if (kv->kv_heads == 0 || kv->kv_heads > 1024u) return "cache: 1 to 1024 kv heads";
+    if ((uint64_t)kv->pages * kv->page * kv->kv_heads >= (1ull << 31)) return "cache: slots * kv heads below 2^31";
     if (!moe_at16(kv->k) || !moe_at16(kv->v)) return "cache: k and v at 16-byte addresses";
     if (kv->type == MOE_KV_E4M3 && (!moe_at16(kv->k_scale) || !moe_at16(kv->v_scale))) return "cache: e4m3 needs scales, at 16-byte addresses";
     return NULL;
@@ -91,7 +92,7 @@ static inline const char *moe_attn_decode_refusal(const moe_cuda_kv_t *kv, const
     if (why != NULL) return why;
     if (!moe_stride_ok(pc.q_stride, (uint64_t)pc.heads * kv->hd) || !moe_stride_ok(pc.o_stride, (uint64_t)pc.heads * kv->hd))
         return "attn_decode: strides are multiples of 8 and hold all heads";
-    if (pc.seqs >= (1u << 20)) return "attn_decode: seqs below 2^20";
+    if (pc.seqs >= (1u << 20) || (uint64_t)pc.seqs * pc.heads >= (1ull << 31)) return "attn_decode: seqs below 2^20, seqs * heads below 2^31";
     if ((uint64_t)pc.table_stride * kv->page < pc.max_len || pc.max_len >= (1u << 31)) return "attn_decode: max_len needs more pages than a row of the table has";
     if (!(pc.scale > 0.0f && pc.scale <= 1.0e4f)) return "attn_decode: scale is positive, 10^4 at most";
     if (pc.seqs != 0 && (!moe_at16(q16) || !moe_at16(o16) || !moe_at4(len) || (pc.max_len != 0 && !moe_at4(table))))

@@ -307,10 +307,11 @@ typedef CUresult (*moe_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   CUtensorMapFloatOOBfill);
 
 static bool moe_encode(moe_cuda_ctx *c, CUtensorMap *out, uint32_t rank, const void *ptr, const cuuint64_t *dims,
-                       const cuuint64_t *strides, const cuuint32_t *box) {
+                       const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                       CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     static const cuuint32_t ones[4] = {1, 1, 1, 1};
-    CUresult r = ((moe_encode_fn)c->encode_tiled)(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, (void *)ptr, dims, strides, box, ones,
-                                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    CUresult r = ((moe_encode_fn)c->encode_tiled)(out, type, rank, (void *)ptr, dims, strides, box, ones,
+                                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) moe_fail(c, MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
     return r == CUDA_SUCCESS;
@@ -403,4 +404,13 @@ bool moe_tmap_heads_f16(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint
     const cuuint64_t dims[3] = {hd, heads, rows}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
     const cuuint32_t box[3] = {64, box_heads, box_rows};
     return moe_encode(c, out, 3, ptr, dims, strides, box);
+}
+
+// Rows of `row` bytes without gaps, cut into lines of 64 or 128 bytes: boxes of `box_rows` rows, in shared memory line by line
+// (all rows' first lines, then all rows' second ones), swizzled inside a line.
+bool moe_tmap_bytes(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint64_t rows, uint32_t row, uint32_t line, uint32_t box_rows) {
+    const cuuint64_t dims[3] = {line, rows, row / line}, strides[2] = {row, line};
+    const cuuint32_t box[3] = {line, box_rows, row / line};
+    return moe_encode(c, out, 3, ptr, dims, strides, box, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                      line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }

@@ -1,32 +1,29 @@
 // Attention of one new token per sequence over the paged key-value cache.
 //
 // Bound by HBM: every cached key and value is read once, and a group of g query heads does 2 g operations per fp16 element.
-// The work is a line: sequence by sequence, head by head, stages of 16 SG cached tokens.  Every warp of a full chip takes an
-// equal piece of the line whatever the lengths are, so no SM waits for another, and walks it alone: its loads run through a
-// ring in shared memory that only it uses (each lane copies exactly the 16-byte pieces it will need as matrix fragments,
-// so the ring needs no barriers and no swizzle), and the ring keeps running across the ends of heads and sequences.
-// A (sequence, head) that lies within one warp's piece is written out at once; the others leave their running maximum, sum and
-// unnormalised output in the context's work area, and a second small kernel joins them in the line's order.
+// The work is a line: sequence by sequence, head by head, stages of 16 or 32 cached tokens.  Every warp of a full chip takes an
+// equal piece of the line whatever the lengths are, so no SM waits for another, and walks it alone: its loads (TMA boxes of
+// one page's tokens, swizzled) run through a ring in shared memory that only it uses, with barriers that only it waits at,
+// and keep running across the ends of heads and sequences.  A (sequence, head) that lies within one warp's piece is written
+// out at once; the others leave their running maximum, sum and unnormalised output in the context's work area, and a second
+// small kernel joins them in the line's order.
 //
-// Fragments: scores are computed as S^T = K Q^T (16 tokens x 8 heads x 16 per mma.sync) and outputs as O^T = V^T P^T, so groups
-// of up to 8 heads waste nothing.  The order of K's columns inside a product is free (Q's is the same), and so is the
-// order of V's columns across products; both are chosen such that a lane's operands are contiguous 16 bytes in the cache.
-// P^T comes from S^T's accumulators by an 8x8 transpose (movmatrix).
+// Scores are computed as S^T = K Q^T (16 tokens x 8 heads x 16 columns per mma.sync) and outputs as O^T = V^T P^T, so groups
+// of up to 8 heads waste nothing; P^T comes from S^T's accumulators by an 8x8 transpose (movmatrix).  Operands come from shared
+// memory by ldmatrix: fp16 as they are; of e4m3 a lane gets two pairs of neighbouring columns, which are converted in
+// registers (the order of K's columns inside a product is free, Q's is the same).
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 
 namespace {
 
-using moe_tc::pack_h2;
-using moe_tc::smem_u32;
+using namespace moe_tc;
 
-constexpr uint32_t DEC_WARPS = 8, DEC_THREADS = DEC_WARPS * 32;
 constexpr float LOG2E = 1.4426950408889634f;
 // Weights are exp2(x - max + WEIGHT_SHIFT): 2^10 at most, so that fp16 holds weights down to 2^-34 of the largest.
 constexpr float WEIGHT_SHIFT = 10.0f;
 
 struct DecArgs {
-    const uint8_t *k, *v;
     const float *k_scale, *v_scale;
     const __half *q;
     const uint32_t *table, *len;
@@ -38,6 +35,7 @@ struct DecArgs {
     uint32_t warps;            // of the grid; part of the line that each takes follows from it and the line's length
     float scale;
     uint32_t *status;
+    uint64_t wait_ns;
 };
 
 // Floats of one warp's unfinished head: a multiple of four, so that every one begins at 16 bytes.
@@ -59,21 +57,17 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-template <uint32_t BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool valid) {  // not valid: zeros, nothing is read
-    const uint32_t n = valid ? BYTES : 0u;
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&v)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ uint2 ld_shared8(uint32_t at) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&v)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(at)
+                 : "memory");
 }
 __device__ __forceinline__ float ld_shared_f(uint32_t at) {
     float v;
@@ -86,22 +80,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Sizes of one stage of one warp's ring.
-template <uint32_t HD, bool FP8>
+// Sizes of one stage of one warp's ring, and how many warps share an SM.
+template <uint32_t HD, uint32_t NT, bool FP8>
 struct Stage {
-    static constexpr uint32_t ES = FP8 ? 1 : 2;
-    static constexpr uint32_t SG = HD == 128 && !FP8 ? 1 : 2;       // groups of 16 tokens
+    static constexpr uint32_t WARPS = NT == 2 ? 8 : 12;
+    static constexpr uint32_t THREADS = WARPS * 32;
+    static constexpr uint32_t ROW = HD * (FP8 ? 1 : 2);             // bytes of a token's keys, or values
+    static constexpr uint32_t LINE = ROW > 128 ? 128 : ROW;         // of them in one swizzled line; two halves if ROW is 256
+    static constexpr uint32_t HALVES = ROW / LINE;
+    static constexpr uint32_t SG = ROW == 256 ? 1 : 2;              // groups of 16 tokens
     static constexpr uint32_t TOKENS = 16 * SG;
-    static constexpr uint32_t KP = HD * ES / 64;                    // 16-byte pieces of a K row per lane (4 lanes a row)
-    static constexpr uint32_t VB = HD * ES / 8 > 16 ? 16 : HD * ES / 8;  // bytes of a V piece (8 lanes a row)
-    static constexpr uint32_t VP = HD * ES / 8 / VB;                // V pieces per token and lane
-    static constexpr uint32_t K_BYTES = 2 * KP * 512;               // of 16 tokens
-    static constexpr uint32_t V_BYTES = 4 * VP * VB * 32;
-    static constexpr uint32_t GROUP_BYTES = K_BYTES + V_BYTES + (FP8 ? 128 : 0);
-    static constexpr uint32_t BYTES = SG * GROUP_BYTES;
-    // about 26 KB per warp: eight warps then keep 150 to 200 KB of an SM's shared memory in flight, three times what
-    // HBM's latency asks for
-    static constexpr uint32_t COUNT = 26000 / BYTES;
+    static constexpr uint32_t HALF_BYTES = TOKENS * LINE;
+    static constexpr uint32_t K_BYTES = TOKENS * ROW;
+    static constexpr uint32_t BYTES = 2 * K_BYTES;
+    static constexpr uint32_t SCALES = FP8 ? 2 * TOKENS * 4 : 0;    // keys' scales, then values'
+    static constexpr uint32_t ROOM = 212000 / WARPS / (BYTES + SCALES);
+    static constexpr uint32_t COUNT = ROOM > 4 ? 4 : ROOM;
+    static constexpr uint32_t RING = WARPS * COUNT * BYTES;
+    static constexpr uint32_t SMEM = RING + WARPS * COUNT * SCALES + WARPS * COUNT * 8 + 1024;
 };
 
 // A place on the line: stage `g` of head h of sequence s.
@@ -123,19 +119,48 @@ __device__ __forceinline__ void place_next(const DecArgs &a, Place &p, uint32_t 
     p.len = p.s < a.seqs ? a.len[p.s] : 0u;
 }
 
+// Bounded wait for a stage; false: gave up, the status says so.
+__device__ __forceinline__ bool landed(uint32_t bar, uint32_t parity, const DecArgs &a) {
+    uint32_t spins = 0;
+    uint64_t t0 = 0;
+    bool ok = true;
+    while (!mbar_try_wait(bar, parity)) {
+        spins += 1;
+        if ((spins & 0xffu) != 0) continue;
+        const uint64_t now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > a.wait_ns) {
+            atomicCAS(a.status, 0u, (uint32_t)MOE_ERR_TIMEOUT | (42u << 8));
+            ok = false;
+            break;
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
 // Where the j-th of `warps` pieces of a line of `total` stages begins.
 __device__ __forceinline__ unsigned long long piece_begin(unsigned long long total, uint32_t j, uint32_t warps) {
     return total * j / warps;
 }
 
 template <uint32_t HD, uint32_t NT, bool FP8>
-__global__ void __launch_bounds__(DEC_THREADS, 1) moe_attn_decode_kernel(DecArgs a) {
-    using St = Stage<HD, FP8>;
-    constexpr uint32_t MT = HD / 16, SG = St::SG, PER = St::TOKENS;
-    extern __shared__ __align__(16) uint8_t ring[];
+__global__ void __launch_bounds__(Stage<HD, NT, FP8>::THREADS, 1)
+moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, DecArgs a) {
+    using St = Stage<HD, NT, FP8>;
+    constexpr uint32_t DEC_WARPS = St::WARPS, DEC_THREADS = St::THREADS;
+    constexpr uint32_t MT = HD / 16, KS = HD / 16, SG = St::SG, PER = St::TOKENS;
+    extern __shared__ uint8_t smem_raw[];
     __shared__ unsigned long long before[DEC_THREADS + 1];
     __shared__ unsigned long long warp_sum[DEC_WARPS];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, r = lane >> 2, c = lane & 3u;
+    uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *const my_ring = smem + warp * St::COUNT * St::BYTES;
+    const uint32_t ring0 = smem_u32(my_ring), scales0 = smem_u32(smem) + St::RING + warp * St::COUNT * St::SCALES;
+    const uint32_t bars0 = smem_u32(smem) + St::RING + DEC_WARPS * St::COUNT * St::SCALES + warp * St::COUNT * 8u;
+    if (lane < St::COUNT) {
+        mbar_init(bars0 + lane * 8u, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     moe_pdl_begin();
 
     // ---- the line: stages before each thread's share of the sequences -----------------------------
@@ -196,61 +221,71 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) moe_attn_decode_kernel(DecArgs
         p.len = a.len[p.s];
     }
 
-    const uint32_t ring0 = smem_u32(ring) + warp * St::COUNT * St::BYTES;
-    Place q = p;             // the next stage to load, and the pages of its groups
-    uint32_t to_load = left;
-    uint32_t pg[SG];
+    Place q = p;             // the next stage to load, and the pages of its boxes
+    uint32_t to_load = left, pg[SG];
+    const uint32_t box = a.page < PER ? a.page : PER;   // tokens of one box: a stage, or a page of 16 of a stage of 32
     auto look_up = [&]() {
 #pragma unroll
         for (uint32_t i = 0; i < SG; i += 1) {
-            const uint32_t t = q.g * PER + i * 16u;
-            pg[i] = to_load != 0 && t < q.len ? a.table[(size_t)q.s * a.table_stride + (t >> a.page_shift)] : 0u;
+            const uint32_t t = q.g * PER + i * box;
+            pg[i] = to_load != 0 && i * box < PER && t < q.len ? a.table[(size_t)q.s * a.table_stride + (t >> a.page_shift)] : 0u;
         }
     };
-    uint32_t bad = 0;  // bit to * SG + i: group i of the stage in ring place `to` lies on a refused page
+    uint32_t bad = 0;   // bit to * SG + i: box i of the stage in ring place `to` lies on a refused page
     // Copies of the next stage into ring place `to`.
     auto load = [&](uint32_t to) {
         if (to_load != 0) {
-            const uint32_t dst0 = ring0 + to * St::BYTES;
+            const uint32_t bar = bars0 + to * 8u, dst = ring0 + to * St::BYTES;
+            int32_t row[SG];
+            uint32_t bytes = 0;
 #pragma unroll
             for (uint32_t i = 0; i < SG; i += 1) {
-                const uint32_t t = q.g * PER + i * 16u;
-                const bool page_ok = pg[i] < a.pages;
-                if (!page_ok && lane == 0) moe_deny(a.status, MOE_SITE_PAGE);
-                bad = (bad & ~(1u << (to * SG + i))) | (page_ok ? 0u : 1u << (to * SG + i));
-                const size_t row = ((((size_t)(page_ok ? pg[i] : 0u) * a.kv_heads + q.h) << a.page_shift) + (t & (a.page - 1u)));
-                const uint32_t n = page_ok && t < q.len ? q.len - t : 0u;  // valid tokens from the group's first on
-                const uint32_t dst = dst0 + i * St::GROUP_BYTES;
-#pragma unroll
-                for (uint32_t j = 0; j < 2u * St::KP; j += 1) {
-                    const uint32_t tok = r + 8u * (j / St::KP), piece = (j % St::KP) * 4u + c;
-                    copy_async<16>(dst + (j * 32u + lane) * 16u, a.k + (row + tok) * (HD * St::ES) + piece * 16u, tok < n);
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < 4u * St::VP; j += 1) {
-                    const uint32_t e = j / St::VP, tok = 2u * c + (e & 1u) + (e >> 1) * 8u, piece = (j % St::VP) * 8u + r;
-                    copy_async<St::VB>(dst + St::K_BYTES + (j * 32u + lane) * St::VB, a.v + (row + tok) * (HD * St::ES) + piece * St::VB,
-                                       tok < n);
-                }
-                if (FP8 && lane < 8u) {
-                    const float *from = (lane < 4u ? a.k_scale : a.v_scale) + row + (lane & 3u) * 4u;
-                    copy_async<16>(dst + St::K_BYTES + St::V_BYTES + lane * 16u, from, n != 0);
+                const uint32_t t = q.g * PER + i * box;
+                const bool page_ok = pg[i] < a.pages, there = i * box < PER && t < q.len;
+                if (there && !page_ok && lane == 0) moe_deny(a.status, MOE_SITE_PAGE);
+                bad = (bad & ~(1u << (to * SG + i))) | ((page_ok ? 0u : 1u) << (to * SG + i));
+                row[i] = there && page_ok ? (int32_t)(((pg[i] * a.kv_heads + q.h) << a.page_shift) + (t & (a.page - 1u))) : -1;
+                bytes += row[i] >= 0 ? 2u * box * St::ROW : 0u;
+                if (FP8 && row[i] >= 0 && lane < box / 2u) {
+                    const uint32_t piece = lane % (box / 4u), is_v = lane / (box / 4u);
+                    copy_async16(scales0 + to * St::SCALES + is_v * PER * 4u + i * box * 4u + piece * 16u,
+                                 (is_v != 0 ? a.v_scale : a.k_scale) + row[i] + piece * 4u);
                 }
             }
+            if (elect_one()) {
+                if (bytes != 0) mbar_expect_tx(bar, bytes);
+                else mbar_arrive(bar);
+#pragma unroll
+                for (uint32_t i = 0; i < SG; i += 1) {
+                    if (row[i] < 0) continue;
+                    tma_load_3d(dst + i * box * St::LINE, &tm_k, bar, 0, row[i], 0);
+                    tma_load_3d(dst + St::K_BYTES + i * box * St::LINE, &tm_v, bar, 0, row[i], 0);
+                }
+            }
+            __syncwarp();
             to_load -= 1;
             if (to_load != 0) place_next(a, q, PER);
             look_up();
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (FP8) asm volatile("cp.async.commit_group;" ::: "memory");
     };
     look_up();
 #pragma unroll
     for (uint32_t i = 0; i < St::COUNT - 1u; i += 1) load(i);
 
+    // ldmatrix: lane l gives the address of row l % 8 of matrix l / 8.  Keys: matrices (tokens 0-7, 8-15) x (line piece 2s, 2s + 1);
+    // values: the other way round.  Pieces of 16 bytes lie at piece ^ (row % 8) of a 128-byte line, piece ^ (row / 2 % 4) of a 64-byte one.
+    auto piece_at = [&](uint32_t token, uint32_t piece) { return token * St::LINE + ((piece ^ (St::LINE == 128 ? token & 7u : (token >> 1) & 3u)) << 4); };
+    const uint32_t k_at = piece_at((lane & 7u) + ((lane >> 3) & 1u) * 8u, lane >> 4);
+    const uint32_t v_at = St::K_BYTES + piece_at((lane & 7u) + (lane >> 4) * 8u, (lane >> 3) & 1u);
+    auto line_step = [](uint32_t at, uint32_t s) {   // two pieces on from `at`, s times: other bits of the same line, then the other half
+        constexpr uint32_t PER_LINE = St::LINE / 32u;
+        return (at ^ ((s % PER_LINE) * 32u)) + (s / PER_LINE) * St::HALF_BYTES;
+    };
     const float to_log2 = a.scale * LOG2E;
-    uint32_t qf[NT][HD / 32u][4];   // Q^T fragments: words 2i, 2i+1 feed product i of a piece's pair
+    uint32_t qf[NT][KS][2];
     float o[MT][NT][4], top[NT][2], sum[NT][2];
-    uint32_t place = 0, begun_at = p.g;
+    uint32_t place = 0, phase = 0, begun_at = p.g;
     bool fresh = true;
     while (left != 0) {
         if (fresh) {
@@ -261,15 +296,18 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) moe_attn_decode_kernel(DecArgs
                 const uint32_t head = n * 8u + r;
                 const __half *row = a.q + (size_t)p.s * a.q_stride + (size_t)(p.h * a.group + head) * HD;
 #pragma unroll
-                for (uint32_t j = 0; j < HD / 32u; j += 1) {
-                    // fp16: piece j of 8 columns; e4m3: a piece is 16 columns, j counts its halves
-                    const uint32_t col = FP8 ? ((j / 2u) * 4u + c) * 16u + (j & 1u) * 8u : (j * 4u + c) * 8u;
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (head < a.group) w = *reinterpret_cast<const uint4 *>(row + col);
-                    qf[n][j][0] = w.x;
-                    qf[n][j][1] = w.y;
-                    qf[n][j][2] = w.z;
-                    qf[n][j][3] = w.w;
+                for (uint32_t k = 0; k < KS; k += 1) {
+                    qf[n][k][0] = qf[n][k][1] = 0;
+                    if (head < a.group) {
+                        if (FP8) {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(row + k * 16u + c * 4u);
+                            qf[n][k][0] = w.x;
+                            qf[n][k][1] = w.y;
+                        } else {
+                            qf[n][k][0] = *reinterpret_cast<const uint32_t *>(row + k * 16u + c * 2u);
+                            qf[n][k][1] = *reinterpret_cast<const uint32_t *>(row + k * 16u + 8u + c * 2u);
+                        }
+                    }
                 }
                 top[n][0] = top[n][1] = -INFINITY;
                 sum[n][0] = sum[n][1] = 0.0f;
@@ -281,58 +319,78 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) moe_attn_decode_kernel(DecArgs
             }
         }
         load(place == 0 ? St::COUNT - 1u : place - 1u);  // into the place whose stage has just been used
-        asm volatile("cp.async.wait_group %0;" ::"n"(St::COUNT - 1u) : "memory");
+        if (FP8) asm volatile("cp.async.wait_group %0;" ::"n"(St::COUNT - 1u) : "memory");
+        if (!landed(bars0 + place * 8u, phase, a)) break;
         __syncwarp();
         const uint32_t at = ring0 + place * St::BYTES;
+        // tokens of each group that are there; what their places hold beyond is nobody's and may be anything
+        uint32_t valid[SG];
+        bool all = true;
+#pragma unroll
+        for (uint32_t i = 0; i < SG; i += 1) {
+            const uint32_t t0 = p.g * PER + i * 16u;
+            const bool refused = (bad >> (place * SG + i * 16u / box) & 1u) != 0u;
+            valid[i] = refused || t0 >= p.len ? 0u : min(16u, p.len - t0);
+            all = all && valid[i] == 16u;
+        }
+        if (!all) {   // 0 x NaN is not 0: values that are not there become zeros
+#pragma unroll
+            for (uint32_t i = 0; i < SG; i += 1) {
+                for (uint32_t u = valid[i] * (St::LINE / 16u) + lane; u < St::LINE; u += 32u) {
+#pragma unroll
+                    for (uint32_t h = 0; h < St::HALVES; h += 1)
+                        *reinterpret_cast<uint4 *>(my_ring + place * St::BYTES + St::K_BYTES + h * St::HALF_BYTES + i * 16u * St::LINE + u * 16u) = make_uint4(0, 0, 0, 0);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before a later TMA load writes here
+            __syncwarp();
+        }
 
         // ---- scores: rows r and r + 8 of each group are tokens, columns 2c and 2c + 1 of each n are heads ----
         float x[SG][NT][4], inv[SG][2];
 #pragma unroll
         for (uint32_t i = 0; i < SG; i += 1) {
-            const uint32_t kb = at + i * St::GROUP_BYTES;
             float s[2][NT][4];
 #pragma unroll
             for (uint32_t n = 0; n < NT; n += 1) {
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e += 1) s[0][n][e] = s[1][n][e] = 0.0f;
             }
+            if (!FP8) {
 #pragma unroll
-            for (uint32_t j = 0; j < St::KP; j += 1) {
-                const uint4 lo = ld_shared16(kb + (j * 32u + lane) * 16u), hi = ld_shared16(kb + ((St::KP + j) * 32u + lane) * 16u);
-                const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
-                if (!FP8) {
+                for (uint32_t k = 0; k < KS; k += 1) {
+                    uint32_t f[4];
+                    ldmatrix_x4(f, line_step(at + i * 16u * St::LINE + k_at, k));
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; n += 1) mma_16816(s[k & 1u][n], f[0], f[1], f[2], f[3], qf[n][k][0], qf[n][k][1]);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < KS; k += 2) {   // a line piece is 16 columns: one product each
+                    uint32_t f[4], lo[4], hi[4];
+                    ldmatrix_x4(f, line_step(at + i * 16u * St::LINE + k_at, k / 2u));
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e += 1) e4m3x4_to_h2(f[e], lo[e], hi[e]);
 #pragma unroll
                     for (uint32_t n = 0; n < NT; n += 1) {
-                        mma_16816(s[0][n], l[0], h[0], l[1], h[1], qf[n][j][0], qf[n][j][1]);
-                        mma_16816(s[1][n], l[2], h[2], l[3], h[3], qf[n][j][2], qf[n][j][3]);
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t w = 0; w < 4; w += 1) {  // a word is four columns of the product
-                        const uint32_t a0 = e4m3x2_to_h2(l[w] & 0xffffu), a2 = e4m3x2_to_h2(l[w] >> 16);
-                        const uint32_t a1 = e4m3x2_to_h2(h[w] & 0xffffu), a3 = e4m3x2_to_h2(h[w] >> 16);
-#pragma unroll
-                        for (uint32_t n = 0; n < NT; n += 1) {
-                            const uint32_t f = (w & 1u) * 2u;
-                            mma_16816(s[w & 1u][n], a0, a1, a2, a3, qf[n][2u * j + w / 2u][f], qf[n][2u * j + w / 2u][f + 1u]);
-                        }
+                        mma_16816(s[0][n], lo[0], lo[1], hi[0], hi[1], qf[n][k][0], qf[n][k][1]);
+                        mma_16816(s[1][n], lo[2], lo[3], hi[2], hi[3], qf[n][k + 1u][0], qf[n][k + 1u][1]);
                     }
                 }
             }
-            const uint32_t t0 = p.g * PER + i * 16u;
 #pragma unroll
             for (uint32_t half = 0; half < 2; half += 1) {
                 float ks = to_log2, lv = 0.0f;
                 inv[i][half] = 1.0f;
                 if (FP8) {
-                    const uint32_t sc = kb + St::K_BYTES + St::V_BYTES + (r + 8u * half) * 4u;
-                    const float vs = ld_shared_f(sc + 64u);
+                    const uint32_t sc = scales0 + place * St::SCALES + (i * 16u + r + 8u * half) * 4u;
+                    const float vs = ld_shared_f(sc + PER * 4u);
                     ks *= ld_shared_f(sc);
                     // V's scale enters as a part of the exponent, so that weights keep their precision whatever the scales are
                     lv = __log2f(vs);
-                    inv[i][half] = __frcp_rn(vs);
+                    inv[i][half] = __fdividef(1.0f, vs);
                 }
-                const bool seen = t0 + r + 8u * half < p.len && (bad >> (place * SG + i) & 1u) == 0u;
+                const bool seen = r + 8u * half < valid[i];
 #pragma unroll
                 for (uint32_t n = 0; n < NT; n += 1) {
 #pragma unroll
@@ -389,96 +447,79 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) moe_attn_decode_kernel(DecArgs
                 }
             }
             // ---- outputs: O^T += V^T P^T, 16 columns of V at a time ----
-            const uint32_t vb = at + i * St::GROUP_BYTES + St::K_BYTES;
-            uint32_t w[4][MT];  // [token 2c, 2c+1, 2c+8, 2c+9][pairs of columns]: first MT / 2 words row r, then row r + 8
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e += 1) {
+            for (uint32_t m = 0; m < MT; m += FP8 ? 2 : 1) {
+                uint32_t f[4];
+                ldmatrix_x4_trans(f, line_step(at + i * 16u * St::LINE + v_at, FP8 ? m / 2u : m));
                 if (!FP8) {
 #pragma unroll
-                    for (uint32_t j = 0; j < St::VP; j += 1) {
-                        const uint4 v = ld_shared16(vb + ((e * St::VP + j) * 32u + lane) * 16u);
-                        w[e][4u * j] = v.x;
-                        w[e][4u * j + 1u] = v.y;
-                        w[e][4u * j + 2u] = v.z;
-                        w[e][4u * j + 3u] = v.w;
-                    }
+                    for (uint32_t n = 0; n < NT; n += 1) mma_16816(o[m][n], f[0], f[1], f[2], f[3], pf[n][0], pf[n][1]);
                 } else {
-                    uint32_t v[4];
-                    if (HD == 128) {
-                        const uint4 y = ld_shared16(vb + (e * 32u + lane) * 16u);
-                        v[0] = y.x;
-                        v[1] = y.y;
-                        v[2] = y.z;
-                        v[3] = y.w;
-                    } else {
-                        const uint2 y = ld_shared8(vb + (e * 32u + lane) * 8u);
-                        v[0] = y.x;
-                        v[1] = y.y;
-                    }
+                    // a lane has columns 2r, 2r + 1 of two tokens: sorted by column and converted, row r and row r + 8 of the product
+                    uint32_t lo[4], hi[4];
 #pragma unroll
-                    for (uint32_t j = 0; j < MT / 2u; j += 1) {
-                        w[e][2u * j] = e4m3x2_to_h2(v[j] & 0xffffu);
-                        w[e][2u * j + 1u] = e4m3x2_to_h2(v[j] >> 16);
+                    for (uint32_t e = 0; e < 4; e += 1) e4m3x4_to_h2(__byte_perm(f[e], 0u, 0x3120u), lo[e], hi[e]);
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; n += 1) {
+                        mma_16816(o[m][n], lo[0], hi[0], lo[2], hi[2], pf[n][0], pf[n][1]);
+                        mma_16816(o[m + 1u][n], lo[1], hi[1], lo[3], hi[3], pf[n][0], pf[n][1]);
                     }
                 }
-            }
-#pragma unroll
-            for (uint32_t m = 0; m < MT; m += 1) {
-                const uint32_t sel = (m & 1u) != 0 ? 0x7632u : 0x5410u;
-                const uint32_t a0 = __byte_perm(w[0][m / 2u], w[1][m / 2u], sel), a1 = __byte_perm(w[0][MT / 2u + m / 2u], w[1][MT / 2u + m / 2u], sel);
-                const uint32_t a2 = __byte_perm(w[2][m / 2u], w[3][m / 2u], sel), a3 = __byte_perm(w[2][MT / 2u + m / 2u], w[3][MT / 2u + m / 2u], sel);
-#pragma unroll
-                for (uint32_t n = 0; n < NT; n += 1) mma_16816(o[m][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
             }
         }
 
         // ---- the end of this head, or of the warp's piece ----
         left -= 1;
-        place = place + 1u == St::COUNT ? 0u : place + 1u;
+        place += 1;
+        if (place == St::COUNT) {
+            place = 0;
+            phase ^= 1u;
+        }
         const bool head_ends = p.g + 1u == p.stages;
         if (head_ends || left == 0) {
             fresh = true;
             const bool whole = head_ends && begun_at == 0;
-            // columns of row half f and tile m: fp16 at 128 columns f * 64 + r * 8 + m, else r * HD/8 + f * HD/16 + m
-            const uint32_t col0 = r * (HD == 128 && !FP8 ? 8u : HD / 8u), colf = HD == 128 && !FP8 ? 64u : HD / 16u;
 #pragma unroll
             for (uint32_t n = 0; n < NT; n += 1) {
+                float l[2];
 #pragma unroll
                 for (uint32_t e = 0; e < 2; e += 1) {
-                    float l = sum[n][e];
-                    l += __shfl_xor_sync(0xffffffffu, l, 4);
-                    l += __shfl_xor_sync(0xffffffffu, l, 8);
-                    l += __shfl_xor_sync(0xffffffffu, l, 16);
-                    const uint32_t head = n * 8u + 2u * c + e;
-                    if (head >= a.group) continue;
-                    if (whole) {
-                        const float f = l == 0.0f ? 0.0f : 1.0f / l;
-                        __half *out = a.o + (size_t)p.s * a.o_stride + (size_t)(p.h * a.group + head) * HD + col0;
+                    l[e] = sum[n][e];
+                    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
+                    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
+                    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
+                }
+                if (whole) {
+                    // transposed back, a lane has two neighbouring columns of head r; of e4m3 the tile's rows 8-15 are its odd columns
+                    const float f0 = l[0] == 0.0f ? 0.0f : 1.0f / l[0], f1 = l[1] == 0.0f ? 0.0f : 1.0f / l[1];
+                    const uint32_t head = n * 8u + r;
+                    __half *out = a.o + (size_t)p.s * a.o_stride + (size_t)(p.h * a.group + head) * HD;
 #pragma unroll
-                        for (uint32_t half = 0; half < 2; half += 1) {
-#pragma unroll
-                            for (uint32_t m = 0; m < MT; m += 4) {
-                                *reinterpret_cast<uint2 *>(out + half * colf + m) =
-                                    make_uint2(pack_h2(o[m][n][half * 2u + e] * f, o[m + 1u][n][half * 2u + e] * f),
-                                               pack_h2(o[m + 2u][n][half * 2u + e] * f, o[m + 3u][n][half * 2u + e] * f));
-                            }
+                    for (uint32_t m = 0; m < MT; m += 1) {
+                        uint32_t y0 = transpose_8x8(pack_h2(o[m][n][0] * f0, o[m][n][1] * f1)), y1 = transpose_8x8(pack_h2(o[m][n][2] * f0, o[m][n][3] * f1));
+                        if (head >= a.group) continue;
+                        if (FP8) {
+                            *reinterpret_cast<uint2 *>(out + m * 16u + c * 4u) = make_uint2(__byte_perm(y0, y1, 0x5410u), __byte_perm(y0, y1, 0x7632u));
+                        } else {
+                            *reinterpret_cast<uint32_t *>(out + m * 16u + c * 2u) = y0;
+                            *reinterpret_cast<uint32_t *>(out + m * 16u + 8u + c * 2u) = y1;
                         }
-                    } else {
-                        // place 0: the piece began inside this head; place 1: the head goes on in the next warp's piece
-                        float *part = a.part + (size_t)(me * 2u + (begun_at == 0 ? 1u : 0u)) * part_floats(a.group, HD);
+                    }
+                } else {
+                    // place 0: the piece began inside this head; place 1: the head goes on in the next warp's piece
+                    float *part = a.part + (size_t)(me * 2u + (begun_at == 0 ? 1u : 0u)) * part_floats(a.group, HD);
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; e += 1) {
+                        const uint32_t head = n * 8u + 2u * c + e;
+                        if (head >= a.group) continue;
                         if (r == 0) {
                             part[a.group * HD + head] = top[n][e];
-                            part[a.group * (HD + 1u) + head] = l;
+                            part[a.group * (HD + 1u) + head] = l[e];
                         }
-                        part += head * HD + col0;
 #pragma unroll
-                        for (uint32_t half = 0; half < 2; half += 1) {
-#pragma unroll
-                            for (uint32_t m = 0; m < MT; m += 4) {
-                                *reinterpret_cast<float4 *>(part + half * colf + m) =
-                                    make_float4(o[m][n][half * 2u + e], o[m + 1u][n][half * 2u + e], o[m + 2u][n][half * 2u + e],
-                                                o[m + 3u][n][half * 2u + e]);
-                            }
+                        for (uint32_t m = 0; m < MT; m += 1) {
+                            part[head * HD + m * 16u + (FP8 ? 2u * r : r)] = o[m][n][e];
+                            part[head * HD + m * 16u + (FP8 ? 2u * r + 1u : r + 8u)] = o[m][n][2u + e];
                         }
                     }
                 }
@@ -486,20 +527,30 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) moe_attn_decode_kernel(DecArgs
         }
         if (left != 0) place_next(a, p, PER);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (FP8) asm volatile("cp.async.wait_all;" ::: "memory");
+    if (left != 0) {   // gave up: a bounded time for the copies in flight
+        for (uint32_t spin = 0; spin < (1u << 16); spin += 1) {
+            bool done = true;
+            for (uint32_t i = 0; i < St::COUNT; i += 1) done = mbar_try_wait(bars0 + i * 8u, i >= place ? phase : phase ^ 1u) && done;
+            if (done) break;
+        }
+    }
 }
 
-// One block per (sequence, kv head): joins the pieces of a head that several warps worked on, in the line's order, and writes
-// zeros for an empty sequence.
+// One block per (sequence, query head): joins the pieces of a head that several warps worked on -- each warp of the block every
+// eighth piece, then the warps' sums, always in the line's order -- and writes zeros for an empty sequence.
+constexpr uint32_t JOIN_WARPS = 8;
 template <uint32_t HD>
-__global__ void __launch_bounds__(128) moe_attn_join_kernel(DecArgs a) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) moe_attn_join_kernel(DecArgs a) {
+    __shared__ float4 y_of[JOIN_WARPS][HD / 4];
+    __shared__ float sum_of[JOIN_WARPS];
     moe_pdl_begin();
-    const uint32_t s = blockIdx.x / a.kv_heads, h = blockIdx.x - s * a.kv_heads;
+    const uint32_t heads = a.kv_heads * a.group, s = blockIdx.x / heads, qh = blockIdx.x - s * heads, h = qh / a.group, head = qh - h * a.group;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const unsigned long long b0 = a.base[s], stages = a.base[s + 1u] - b0;
-    __half *out = a.o + (size_t)s * a.o_stride + (size_t)h * a.group * HD;
-    const uint32_t units = a.group * HD / 4u;
+    __half *out = a.o + (size_t)s * a.o_stride + (size_t)qh * HD;
     if (stages == 0) {
-        for (uint32_t u = threadIdx.x; u < units; u += blockDim.x) *reinterpret_cast<uint2 *>(out + u * 4u) = make_uint2(0, 0);
+        if (threadIdx.x < HD / 4u) *reinterpret_cast<uint2 *>(out + threadIdx.x * 4u) = make_uint2(0, 0);
         return;
     }
     const unsigned long long total = a.base[a.seqs] * a.kv_heads, x0 = b0 * a.kv_heads + h * stages, x1 = x0 + stages;
@@ -507,40 +558,64 @@ __global__ void __launch_bounds__(128) moe_attn_join_kernel(DecArgs a) {
     // the piece that holds x: the largest j with total * j / warps <= x
     const uint32_t w0 = (uint32_t)(((x0 + 1u) * warps - 1u) / total), w1 = (uint32_t)((x1 * warps - 1u) / total);
     if (w0 == w1) return;
-    const uint32_t size = part_floats(a.group, HD);
-    for (uint32_t u = threadIdx.x; u < units; u += blockDim.x) {
-        const uint32_t head = u / (HD / 4u);
-        float top = -INFINITY;
-        for (uint32_t w = w0; w <= w1; w += 1) top = fmaxf(top, a.part[(size_t)(w * 2u + (w == w0 ? 1u : 0u)) * size + a.group * HD + head]);
-        float sum = 0.0f;
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const uint32_t size = part_floats(a.group, HD), n = w1 - w0 + 1u;
+    auto piece = [&](uint32_t i) { return a.part + (size_t)((w0 + i) * 2u + (i == 0 ? 1u : 0u)) * size; };
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < n; i += 32u) top = fmaxf(top, piece(i)[a.group * HD + head]);
+#pragma unroll
+    for (uint32_t o = 16; o != 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const bool mine = lane < HD / 4u;
 #pragma unroll 4
-        for (uint32_t w = w0; w <= w1; w += 1) {
-            const float *part = a.part + (size_t)(w * 2u + (w == w0 ? 1u : 0u)) * size;
-            const float m = part[a.group * HD + head];
-            const float f = m == top ? 1.0f : exp2_fast(m - top);
-            const float4 v = *reinterpret_cast<const float4 *>(part + u * 4u);
-            sum += f * part[a.group * (HD + 1u) + head];
-            y.x += f * v.x;
-            y.y += f * v.y;
-            y.z += f * v.z;
-            y.w += f * v.w;
-        }
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-        *reinterpret_cast<uint2 *>(out + u * 4u) = make_uint2(pack_h2(y.x * f, y.y * f), pack_h2(y.z * f, y.w * f));
+    for (uint32_t i = warp; i < n; i += JOIN_WARPS) {
+        const float *part = piece(i);
+        const float m = part[a.group * HD + head], l = part[a.group * (HD + 1u) + head];
+        const float4 v = *reinterpret_cast<const float4 *>(part + head * HD + (mine ? lane * 4u : 0u));
+        const float f = m == top ? 1.0f : exp2_fast(m - top);
+        sum += f * l;
+        y.x += f * v.x;
+        y.y += f * v.y;
+        y.z += f * v.z;
+        y.w += f * v.w;
     }
+    if (mine) y_of[warp][lane] = y;
+    if (lane == 0) sum_of[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x >= HD / 4u) return;
+    sum = 0.0f;
+    y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t w = 0; w < JOIN_WARPS; w += 1) {
+        const float4 v = y_of[w][threadIdx.x];
+        sum += sum_of[w];
+        y.x += v.x;
+        y.y += v.y;
+        y.z += v.z;
+        y.w += v.w;
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2 *>(out + threadIdx.x * 4u) = make_uint2(pack_h2(y.x * f, y.y * f), pack_h2(y.z * f, y.w * f));
 }
 
 template <uint32_t HD, uint32_t NT, bool FP8>
-void decode_launch(moe_cuda_ctx *c, const DecArgs &a, uint32_t slot) {
-    constexpr uint32_t smem = DEC_WARPS * Stage<HD, FP8>::COUNT * Stage<HD, FP8>::BYTES;
+void decode_launch(moe_cuda_ctx *c, const moe_cuda_kv_t *kv, const DecArgs &args, uint32_t slot) {
+    using St = Stage<HD, NT, FP8>;
+    constexpr uint32_t smem = St::SMEM;
+    static_assert(St::COUNT >= 2 && St::COUNT * St::SG <= 32 && smem + 8192 <= 227 * 1024, "ring");
+    CUtensorMap tk, tv;
+    const uint64_t rows = (uint64_t)kv->pages * kv->kv_heads * kv->page;
+    const uint32_t box = kv->page < St::TOKENS ? kv->page : St::TOKENS;
+    if (!moe_tmap_bytes(c, &tk, kv->k, rows, St::ROW, St::LINE, box) || !moe_tmap_bytes(c, &tv, kv->v, rows, St::ROW, St::LINE, box)) return;
+    DecArgs a = args;
+    a.warps = (uint32_t)c->sm_count * St::WARPS;
     if (!c->dec_attr_set[slot]) {
         MOE_CUDA_TRY(c, cudaFuncSetAttribute(moe_attn_decode_kernel<HD, NT, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         c->dec_attr_set[slot] = true;
     }
-    moe_run(c, moe_attn_decode_kernel<HD, NT, FP8>, (uint32_t)c->sm_count, DEC_THREADS, smem, a);
+    moe_run(c, moe_attn_decode_kernel<HD, NT, FP8>, (uint32_t)c->sm_count, St::THREADS, smem, tk, tv, a);
     MOE_LAUNCHED(c);
-    moe_run(c, moe_attn_join_kernel<HD>, a.seqs * a.kv_heads, 128, 0, a);
+    moe_run(c, moe_attn_join_kernel<HD>, a.seqs * a.kv_heads * a.group, JOIN_WARPS * 32, 0, a);
     MOE_LAUNCHED(c);
 }
 
@@ -553,8 +628,6 @@ extern "C" void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv,
     MOE_REQUIRE(c, why == NULL, "%s", why);
     if (pc.seqs == 0) return;
     DecArgs a;
-    a.k = (const uint8_t *)kv->k;
-    a.v = (const uint8_t *)kv->v;
     a.k_scale = kv->k_scale;
     a.v_scale = kv->v_scale;
     a.q = (const __half *)q16;
@@ -571,9 +644,10 @@ extern "C" void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv,
     a.table_stride = pc.table_stride;
     a.q_stride = pc.q_stride;
     a.o_stride = pc.o_stride;
-    a.warps = (uint32_t)c->sm_count * DEC_WARPS;
+    a.warps = (uint32_t)c->sm_count * 16u;   // at most; the variant sets its own
     a.scale = pc.scale;
     a.status = c->dev_status_dev;
+    a.wait_ns = c->wait_ns;
     const size_t base_bytes = (((size_t)pc.seqs + 1u) * 8u + 255u) & ~(size_t)255u;
     const size_t part_bytes = (size_t)a.warps * 2u * part_floats(a.group, kv->hd) * 4u;
     if (base_bytes + part_bytes > c->work_bytes) {
@@ -585,10 +659,10 @@ extern "C" void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv,
     moe_on_device on(c);
     const bool fp8 = kv->type == MOE_KV_E4M3, wide = a.group > 8u;
     if (kv->hd == 128u) {
-        if (fp8) wide ? decode_launch<128, 2, true>(c, a, 0) : decode_launch<128, 1, true>(c, a, 1);
-        else wide ? decode_launch<128, 2, false>(c, a, 2) : decode_launch<128, 1, false>(c, a, 3);
+        if (fp8) wide ? decode_launch<128, 2, true>(c, kv, a, 0) : decode_launch<128, 1, true>(c, kv, a, 1);
+        else wide ? decode_launch<128, 2, false>(c, kv, a, 2) : decode_launch<128, 1, false>(c, kv, a, 3);
     } else {
-        if (fp8) wide ? decode_launch<64, 2, true>(c, a, 4) : decode_launch<64, 1, true>(c, a, 5);
-        else wide ? decode_launch<64, 2, false>(c, a, 6) : decode_launch<64, 1, false>(c, a, 7);
+        if (fp8) wide ? decode_launch<64, 2, true>(c, kv, a, 4) : decode_launch<64, 1, true>(c, kv, a, 5);
+        else wide ? decode_launch<64, 2, false>(c, kv, a, 6) : decode_launch<64, 1, false>(c, kv, a, 7);
     }
 }

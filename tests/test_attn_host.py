@@ -76,7 +76,8 @@ def test_cache_refusals(args, mc, change):
 
 
 def test_cache_takes_all_but_the_last_slots(args, mc):
-    assert args.kv(C.byref(mc.Kv(**{**KV, "pages": 2 ** 28 - 1, "page": 16}))) is None
+    assert args.kv(C.byref(mc.Kv(**{**KV, "pages": 2 ** 27 - 1, "page": 16, "kv_heads": 1}))) is None
+    assert args.kv(C.byref(mc.Kv(**{**KV, "pages": 2 ** 26, "page": 16, "kv_heads": 2}))) is not None
 
 
 @pytest.mark.parametrize("rows,stride,at", [(3, 120, (AT, AT, AT)), (3, 132, (AT, AT, AT)), (2 ** 29, 128, (AT, AT, AT)), (3, 128, (None, AT, AT)),
