@@ -8,16 +8,23 @@
 // its keys and values once, and a tile spans few tokens, which keeps what is computed above the diagonal small.  A CTA works
 // on two such tiles (256 rows) against the same key blocks of 128, so that one tile's softmax runs under the other's products.
 // Persistent CTAs, one per SM, walk a list of (tile pair, kv head), the longest first.  Roles:
-//   warp 0     loads Q (both tiles) and K blocks by TMA            warp 3   loads V blocks
-//   warp 1     issues every tcgen05.mma: S of both tiles into tensor memory, then per block P V into the output accumulator
-//              (P is read from tensor memory, where it overwrites its own S)
+//   warp 0     loads Q (both tiles), K and V blocks by TMA, a block to a load
+//   warps 1, 3 issue the tcgen05.mma of the first and the second tile: S into tensor memory, then per block P V into the output
+//              accumulator (P is read from tensor memory, where it overwrites its own S).  A warp of its own for each tile: a
+//              look at a barrier takes some 200 cycles, and one tile's looks hide under the other's products
 //   warp 2     makes V blocks that some row must not see in part safe (below)
-//   warps 4-7, 8-11   softmax of the first and second tile, a row per thread; rescale and write the output
-// The output accumulator is rescaled only when a row's maximum has grown by more than 2^6; until then weights are taken against
-// the older maximum, which stays inside fp16's range.
+//   warps 4-7, 8-11   softmax of the first and second tile, a row per thread
+//   warps 12-15       scale and store the finished output of both tiles, while the softmax is at the next item
+// What a tile waits for is softmax, then its products, then softmax again; so the softmax's own time counts, not only its
+// throughput.  It takes scores two at a time where it can (f32x2 arithmetic, maxima of three), hands P over in two halves, and
+// leaves a share of the exponentials to the multiply-add pipe: 2^x = 2^n * 2^f with n the nearest integer and a polynomial of
+// degree 4 in f (fitted for the least relative error on [-1/2, 1/2], 2^-18.5, seven bits below P's rounding).
+// The output accumulator is rescaled, by the softmax warps, only when a row's maximum has grown by more than 2^6; until then
+// weights are taken against the older maximum, which stays inside fp16's range.
 // A masked weight is 0, but 0 x NaN and 0 x infinity are not.  So the blocks that reach over the diagonal or the sequence's
 // end are looked through before their product: their non-finite values become 0 in shared memory, and if there were any,
 // the rows that do see them get them added at the end from global memory (a weight is positive, so infinities keep their sign).
+// A NaN score makes the row's maximum NaN, and with it the whole row.
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 
@@ -25,11 +32,13 @@ namespace {
 
 using namespace moe_tc;
 
-constexpr uint32_t AT_THREADS = 384, TILE_ROWS = 128, BLOCK_KEYS = 128;
+constexpr uint32_t AT_THREADS = 512, TILE_ROWS = 128, BLOCK_KEYS = 128;
 constexpr uint32_t HALF_BYTES = 128 * 128;       // 128 rows of 64 columns, one TMA box
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float GROW = 6.0f;                     // log2 of how far weights may pass the reference before a rescale
 constexpr float SHIFT = 8.0f;                    // weights are at most 2^(GROW + SHIFT) = 2^14; fp16 then goes down to 2^-32 of the reference
+// Of every POLY_OF pairs of exponentials POLY_SHARE go to the multiply-add pipe.
+constexpr uint32_t POLY_OF = 4, POLY_SHARE = 1;
 constexpr uint32_t FLAGS = 8;                    // items that may be between their V check and their epilogue
 
 template <uint32_t HD>
@@ -45,10 +54,13 @@ struct __align__(8) AttnBars {
     uint64_t kv_full[ST], kv_empty[ST];
     uint64_t v_landed[ST];   // masked V blocks: loaded; warp 2 then arrives at kv_full
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
-    uint64_t drain;          // unwinding: all products issued have retired
+    uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];   // p_full: of each tile, keys 0-63 and 64-127
+    uint64_t sum_full[2], sum_empty[2];
+    uint64_t turn[2];        // the tile's softmax may begin: the other one's has ended
+    uint64_t drain[2];       // unwinding: all products issued have retired
     uint32_t tmem_base, abort;
     uint32_t found[FLAGS];   // the item's masked V blocks held something that is not finite
+    float sum[2][TILE_ROWS];
 };
 
 // A pair of tiles of one sequence: `left` queries from row q_row on, the sequence's keys from row k_row on.
@@ -77,7 +89,9 @@ __device__ __forceinline__ uint32_t span(uint32_t a, uint32_t b, uint32_t rows) 
 // What a CTA has to do, in turn: round r takes item r * G + c, odd rounds from the other end, so that with falling costs every
 // CTA gets about the same.
 struct Items {
-    uint32_t count, round;
+    uint32_t count, round, head;
+    Pair p;            // of the next item, loaded one item ahead
+    bool more;
     Pair one;
     uint32_t one_pairs;
 
@@ -93,15 +107,13 @@ struct Items {
         } else {
             count = *a.pairs * a.kv_heads;
         }
+        fetch(a);
     }
-    __device__ __forceinline__ bool next(const AttnArgs &a, Pair &p, uint32_t &head) {
+    __device__ __forceinline__ void fetch(const AttnArgs &a) {
         const uint32_t at = round * gridDim.x + ((round & 1u) != 0 ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
-        if (at >= count) return false;   // a round that is too short for this CTA is the last one
+        more = at < count;   // a round that is too short for this CTA is the last one
+        if (!more) return;
         round += 1;
-        take(a, at, p, head);
-        return true;
-    }
-    __device__ __forceinline__ void take(const AttnArgs &a, uint32_t at, Pair &p, uint32_t &head) {
         const uint32_t i = at / a.kv_heads;
         head = at - i * a.kv_heads;
         if (a.plan == nullptr) {
@@ -117,6 +129,13 @@ struct Items {
             p.k_row = e.z;
             p.lk = e.w;
         }
+    }
+    __device__ __forceinline__ bool next(const AttnArgs &a, Pair &now, uint32_t &now_head) {
+        if (!more) return false;
+        now = p;
+        now_head = head;
+        fetch(a);
+        return true;
     }
 };
 
@@ -156,6 +175,23 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         : "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
         : "memory");
 }
+// A box of some heads of some rows, from 64-column half `half` on.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t head, int32_t row, int32_t half = 0) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        :
+        : "r"(dst), "l"((uint64_t)map), "r"(bar), "r"(0), "r"(head), "r"(row), "r"(half)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -175,11 +211,76 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         "r"(v[31])
         : "memory");
 }
+// Waits for this thread's loads; what was loaded into v is used behind it only.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                   "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                   "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                   "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+__device__ __forceinline__ float max_nan(float x, float y, float z) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
+// Two fp32 values in one register pair.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void apart(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+// 2^x for two x below 127 (what lies below -126 counts as -126); not for NaN.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float &y0, float &y1) {
+    float a, b;
+    apart(x, a, b);
+    x = two(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t magic = two(12582912.0f, 12582912.0f), minus = two(-12582912.0f, -12582912.0f), one = two(-1.0f, -1.0f);
+    const uint64_t t = add2(x, magic);                  // the nearest integer in the low bits
+    const uint64_t f = fma2(add2(t, minus), one, x);    // [-1/2, 1/2]
+    uint64_t v = fma2(two(0.0095701f, 0.0095701f), f, two(0.05591786f, 0.05591786f));
+    v = fma2(v, f, two(0.24024745f, 0.24024745f));
+    v = fma2(v, f, two(0.69312181f, 0.69312181f));
+    v = fma2(v, f, two(0.99999926f, 0.99999926f));
+    float n0, n1;
+    apart(t, n0, n1);
+    apart(v, y0, y1);
+    y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(n0) << 23));
+    y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(n1) << 23));
+}
+__device__ __forceinline__ void store32(__half *to, const uint32_t (&w)[8], bool whole) {   // 32 bytes, at once if they are aligned
+    if (whole) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                     "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4 *>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
 }
 
 // mbar_wait without a call, so that the registers of a softmax thread need not follow a calling convention.
@@ -218,15 +319,19 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < ST; i += 1) {
             mbar_init(smem_u32(&bars->kv_full[i]), 1);
-            mbar_init(smem_u32(&bars->kv_empty[i]), 1);
+            mbar_init(smem_u32(&bars->kv_empty[i]), 2);
             mbar_init(smem_u32(&bars->v_landed[i]), 1);
         }
         mbar_init(smem_u32(&bars->q_full), 1);
-        mbar_init(smem_u32(&bars->q_empty), 1);
-        mbar_init(smem_u32(&bars->drain), 1);
+        mbar_init(smem_u32(&bars->q_empty), 2);
         for (uint32_t i = 0; i < 2; i += 1) {
             mbar_init(smem_u32(&bars->s_full[i]), 1);
-            mbar_init(smem_u32(&bars->p_full[i]), TILE_ROWS);
+            mbar_init(smem_u32(&bars->p_full[i][0]), TILE_ROWS);
+            mbar_init(smem_u32(&bars->p_full[i][1]), TILE_ROWS);
+            mbar_init(smem_u32(&bars->sum_full[i]), TILE_ROWS);
+            mbar_init(smem_u32(&bars->sum_empty[i]), TILE_ROWS);
+            mbar_init(smem_u32(&bars->turn[i]), 4);
+            mbar_init(smem_u32(&bars->drain[i]), 1);
             mbar_init(smem_u32(&bars->o_full[i]), 1);
             mbar_init(smem_u32(&bars->o_empty[i]), TILE_ROWS);
         }
@@ -240,7 +345,8 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bars->tmem_base;   // S of the two tiles at 0 and 128, O at 256 and 256 + HD
+    // all 512 columns are this CTA's, so they begin at 0
+    constexpr uint32_t tmem = 0;   // S of the two tiles at 0 and 128, O at 256 and 256 + HD
 
     moe_pdl_begin();
 
@@ -254,34 +360,33 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         (a.cu_q[0] > a.cu_q[1] || a.cu_q[1] > a.rows_q || a.cu_k[0] > a.cu_k[1] || a.cu_k[1] > a.rows_k)) {
         moe_deny(a.status, MOE_SITE_ROWS);
     }
-    // 384 threads start with 168 registers: the softmax keeps a whole row of scores in them, the other warps need few
     if (warp < 4u) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 0 || warp == 3) {
+        if (warp == 0) {
             // ---------------- loads: ring places K(n-1), V(n-1), K(n-2), V(n-2), ... of each item in turn ----------------
             if (lane == 0) {
-                const bool is_v = warp == 3;
-                uint32_t at = is_v ? 1u : 0u, q_phase = 1, issued = 0, parity = 0, masked = 0, landed = 0;
-                uint32_t q_bytes = 0, q_loads = 0;
+                uint32_t at = 0, q_phase = 1, issued = 0, parity = 0, masked = 0, landed = 0, q_loads = 0;
                 bool ok = true;
                 while (ok && items.next(a, p, head)) {
                     const Blocks b = blocks_of(p, a.tile_tokens);
                     if (b.n == 0) continue;
-                    if (!is_v) {
-                        if (!AT_WAIT(&bars->q_empty, q_phase, 31)) break;
-                        q_phase ^= 1u;
-                        q_bytes = a.group * a.tile_tokens * 128u * C::HALVES * (b.has_b ? 2u : 1u);
-                        mbar_expect_tx(smem_u32(&bars->q_full), q_bytes);
-                        for (uint32_t t = 0; t < (b.has_b ? 2u : 1u); t += 1) {
-                            for (uint32_t h = 0; h < C::HALVES; h += 1) {
-                                tma_load_3d(q_smem + t * C::TILE_BYTES + h * HALF_BYTES, &tm_q, smem_u32(&bars->q_full), (int32_t)(h * 64u),
-                                            (int32_t)(head * a.group), (int32_t)(p.q_row + t * a.tile_tokens));
+                    for (uint32_t i = 0; i < 2u * b.n; i += 1) {
+                        const uint32_t j = b.n - 1u - i / 2u, s = at % ST, ph = (at / ST) & 1u;
+                        const bool is_v = (i & 1u) != 0;
+                        if (i == 0) {
+                            if (!AT_WAIT(&bars->q_empty, q_phase, 31)) {
+                                ok = false;
+                                break;
                             }
+                            q_phase ^= 1u;
+                            mbar_expect_tx(smem_u32(&bars->q_full), a.group * a.tile_tokens * HD * 2u * (b.has_b ? 2u : 1u));
+                            // a group of an odd size leaves rows of the tile free, so each half is placed by itself
+                            for (uint32_t x = 0; x < (b.has_b ? 2u : 1u) * C::HALVES; x += 1) {
+                                const uint32_t tile = x / C::HALVES, half = x % C::HALVES;
+                                tma_load_4d(q_smem + tile * C::TILE_BYTES + half * HALF_BYTES, &tm_q, smem_u32(&bars->q_full),
+                                            (int32_t)(head * a.group), (int32_t)(p.q_row + tile * a.tile_tokens), (int32_t)half);
+                            }
+                            q_loads += 1;
                         }
-                        q_loads += 1;
-                    }
-                    for (uint32_t j = b.n; j-- > 0;) {
-                        const uint32_t s = at % ST, ph = (at / ST) & 1u;
                         if (!AT_WAIT(&bars->kv_empty[s], ph ^ 1u, 32)) {
                             ok = false;
                             break;
@@ -289,15 +394,12 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                         const bool m = is_v && (int32_t)j >= b.masked_from;
                         const uint32_t full = smem_u32(m ? &bars->v_landed[s] : &bars->kv_full[s]);
                         mbar_expect_tx(full, C::TILE_BYTES);
-                        for (uint32_t h = 0; h < C::HALVES; h += 1) {
-                            tma_load_3d(ring + s * C::TILE_BYTES + h * HALF_BYTES, is_v ? &tm_v : &tm_k, full, (int32_t)(h * 64u), (int32_t)head,
-                                        (int32_t)(p.k_row + j * BLOCK_KEYS));
-                        }
+                        tma_load_4d(ring + s * C::TILE_BYTES, is_v ? &tm_v : &tm_k, full, (int32_t)head, (int32_t)(p.k_row + j * BLOCK_KEYS));
                         issued |= 1u << s;
                         parity = (parity & ~(1u << s)) | (ph << s);
                         masked = (masked & ~(1u << s)) | ((m ? 1u : 0u) << s);
                         landed ^= (m ? 1u : 0u) << s;   // the next masked use's parity
-                        at += 2u;
+                        at += 1u;
                     }
                 }
                 if (*abort != 0) {
@@ -317,90 +419,83 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 }
             }
             __syncwarp();
-        } else if (warp == 1) {
-            // ---------------- MMA issue: the whole warp runs the loop, one elected lane issues ----------------
-            uint32_t at = 0, q_phase = 0, p_phase = 0, o_phase = 3;
+        } else if (warp == 1 || warp == 3) {
+            // ---------------- MMA issue: a whole warp runs each tile's loop, one elected lane issues ----------------
+            const uint32_t t = warp >> 1;
+            const uint32_t s_at = tmem + t * 128u, o_at = tmem + 256u + t * HD;
+            const uint64_t qd = umma_desc(q_smem + t * C::TILE_BYTES);
+            uint32_t at = 0, q_phase = 0, p_phase = 0, o_phase = 1;
             bool ok = true;
             const uint32_t idesc_s = umma_idesc(128, BLOCK_KEYS), idesc_o = umma_idesc(128, HD) | (1u << 16);  // V: MN-major
-            auto scores = [&](uint32_t t, uint32_t slot) {
+            // S of the block in ring place `slot`; last: the item's last use of Q
+            auto scores = [&](uint32_t slot, bool mine, bool last) {
+                tc_fence_after();
                 if (elect_one()) {
-                    const uint64_t qd = umma_desc(q_smem + t * C::TILE_BYTES), kd = umma_desc(ring + slot * C::TILE_BYTES);
+                    if (mine) {
+                        const uint64_t kd = umma_desc(ring + slot * C::TILE_BYTES);
 #pragma unroll
-                    for (uint32_t k = 0; k < HD / 16u; k += 1) {
-                        const uint64_t off = (uint64_t)((k / 4u) * (HALF_BYTES >> 4) + (k % 4u) * 2u);
-                        umma_f16(tmem + t * 128u, qd + off, kd + off, idesc_s, k != 0 ? 1u : 0u);
+                        for (uint32_t k = 0; k < HD / 16u; k += 1) {
+                            const uint64_t off = (uint64_t)((k / 4u) * (HALF_BYTES >> 4) + (k % 4u) * 2u);
+                            umma_f16(s_at, qd + off, kd + off, idesc_s, k != 0 ? 1u : 0u);
+                        }
+                        umma_commit(smem_u32(&bars->s_full[t]));
                     }
-                    umma_commit(smem_u32(&bars->s_full[t]));
+                    umma_commit(smem_u32(&bars->kv_empty[slot]));
+                    if (last) umma_commit(smem_u32(&bars->q_empty));
                 }
                 __syncwarp();
             };
             while (ok && items.next(a, p, head)) {
                 const Blocks b = blocks_of(p, a.tile_tokens);
                 if (b.n == 0) continue;
-                if (!AT_WAIT(&bars->q_full, q_phase, 33)) break;
-                q_phase ^= 1u;
                 uint32_t ks = at % ST;
-                if (!AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34)) break;
+                ok = AT_WAIT(&bars->q_full, q_phase, 33) && AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34);
                 __syncwarp();
-                tc_fence_after();
-                for (uint32_t t = 0; t < 2; t += 1) {
-                    if (b.n == b.tile[t]) scores(t, ks);
-                }
-                if (elect_one()) {
-                    umma_commit(smem_u32(&bars->kv_empty[ks]));
-                    if (b.n == 1u) umma_commit(smem_u32(&bars->q_empty));
-                }
-                __syncwarp();
-                for (uint32_t j = b.n; j-- > 0 && ok;) {
+                if (!ok) break;
+                q_phase ^= 1u;
+                scores(ks, b.n == b.tile[t], b.n == 1u);
+                for (uint32_t j = b.n; j-- > 0;) {
                     const uint32_t vi = at + 1u, vs = vi % ST;
-                    ok = AT_WAIT(&bars->kv_full[vs], (vi / ST) & 1u, 35);
                     at += 2u;
                     ks = at % ST;
-                    if (ok && j != 0) ok = AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34);
-                    for (uint32_t t = 0; t < 2u && ok; t += 1) {
-                        if (j < b.tile[t]) {
-                            const bool first = j + 1u == b.tile[t];
-                            if (first) {
-                                ok = AT_WAIT(&bars->o_empty[t], o_phase >> t & 1u, 37);
-                                o_phase ^= 1u << t;
-                            }
-                            ok = ok && AT_WAIT(&bars->p_full[t], p_phase >> t & 1u, 38);
-                            p_phase ^= 1u << t;
-                            if (!ok) break;
-                            __syncwarp();
-                            tc_fence_after();
-                            if (elect_one()) {
-                                const uint64_t vd = v_desc(ring + vs * C::TILE_BYTES);
+                    ok = AT_WAIT(&bars->kv_full[vs], (vi / ST) & 1u, 35) && (j == 0 || AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34));
+                    if (j < b.tile[t]) {
+                        const bool first = j + 1u == b.tile[t];
+                        if (first) {
+                            ok = ok && AT_WAIT(&bars->o_empty[t], o_phase, 37);
+                            o_phase ^= 1u;
+                        }
 #pragma unroll
-                                for (uint32_t k = 0; k < BLOCK_KEYS / 16u; k += 1) {
-                                    umma_f16_ts(tmem + 256u + t * HD, tmem + t * 128u + k * 8u, vd + k * 128u, idesc_o, first && k == 0 ? 0u : 1u);
+                        for (uint32_t part = 0; part < 2u; part += 1) {
+                            ok = ok && AT_WAIT(&bars->p_full[t][part], p_phase, 38);
+                            __syncwarp();
+                            tc_fence_after();
+                            if (ok && elect_one()) {
+                                const uint64_t vd = v_desc(ring + vs * C::TILE_BYTES) + part * 512u;
+#pragma unroll
+                                for (uint32_t k = 0; k < BLOCK_KEYS / 32u; k += 1) {
+                                    umma_f16_ts(o_at, s_at + part * 32u + k * 8u, vd + k * 128u, idesc_o, first && part == 0 && k == 0 ? 0u : 1u);
                                 }
-                                if (j == 0) umma_commit(smem_u32(&bars->o_full[t]));
+                                if (j == 0 && part == 1u) umma_commit(smem_u32(&bars->o_full[t]));
                             }
                             __syncwarp();
                         }
-                        if (j != 0 && j - 1u < b.tile[t]) {
-                            __syncwarp();
-                            tc_fence_after();
-                            scores(t, ks);
-                        }
+                        p_phase ^= 1u;
                     }
+                    __syncwarp();
                     if (!ok) break;
-                    if (elect_one()) {
-                        umma_commit(smem_u32(&bars->kv_empty[vs]));
-                        if (j != 0) umma_commit(smem_u32(&bars->kv_empty[ks]));
-                        if (j == 1u) umma_commit(smem_u32(&bars->q_empty));
-                    }
+                    if (j != 0) scores(ks, j - 1u < b.tile[t], j == 1u);
+                    if (elect_one()) umma_commit(smem_u32(&bars->kv_empty[vs]));
                     __syncwarp();
                 }
             }
             __syncwarp();
             if (*abort != 0) {
                 // unwinding: a bounded time for the products already issued
-                if (elect_one()) umma_commit(smem_u32(&bars->drain));
+                if (elect_one()) umma_commit(smem_u32(&bars->drain[t]));
                 __syncwarp();
                 for (uint32_t spin = 0; spin < (1u << 16); spin += 1) {
-                    if (mbar_try_wait(smem_u32(&bars->drain), 0)) break;
+                    if (mbar_try_wait(smem_u32(&bars->drain[t]), 0)) break;
                 }
             }
             __syncwarp();
@@ -424,7 +519,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     __syncwarp();
                     uint8_t *block = smem + (2u + vs) * C::TILE_BYTES;
                     uint32_t most = 0;   // the largest exponent and mantissa of either half
-#pragma unroll 8
+#pragma unroll 4
                     for (uint32_t i = lane; i < C::TILE_BYTES / 16u; i += 32u) {
                         const uint4 w = *reinterpret_cast<const uint4 *>(block + i * 16u);
                         most = __vmaxu2(__vmaxu2(__vmaxu2(most, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, w.z & 0x7fff7fffu)), w.w & 0x7fff7fffu);
@@ -448,31 +543,21 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
             __syncwarp();
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        // ---------------- softmax and output: a row per thread ----------------
+    } else if (warp < 12u) {
+        // ---------------- softmax: a row per thread ----------------
         const uint32_t t = (warp - 4u) >> 2, row = (warp & 3u) * 32u + lane;
-        const uint32_t my_token = row / a.group, my_head = row - my_token * a.group;
+        const uint32_t my_token = row / a.group;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t s_at = tmem + t * 128u + lanes, o_at = tmem + 256u + t * HD + lanes;
         const float to_log2 = a.scale * LOG2E;
-        uint32_t s_phase = 0, o_phase = 0, n_item = 0;
+        const uint64_t scale2 = two(to_log2, to_log2);
+        uint32_t s_phase = 0, sum_phase = 1, turn_phase = t == 0 ? 1u : 0u;   // the first tile begins
         bool ok = true;
         while (ok && items.next(a, p, head)) {
             const Blocks b = blocks_of(p, a.tile_tokens);
-            const uint32_t token = t * a.tile_tokens + my_token;   // behind the pair's first
-            const bool mine = my_token < a.tile_tokens && token < p.left;
-            __half *out = a.o + (size_t)(p.q_row + token) * a.o_stride + (size_t)(head * a.group + my_head) * HD;
-            const uint32_t n = b.tile[t], flag = n_item % FLAGS;
-            if (b.n != 0) n_item += 1;
-            if (n == 0) {   // no query, or none that sees a key
-                if (mine) {
-#pragma unroll
-                    for (uint32_t i = 0; i < HD; i += 8) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
-                }
-                continue;
-            }
-            const int32_t vis = visible(p, token);
+            const uint32_t n = b.tile[t], both = min(b.tile[0], b.tile[1]);   // blocks that both tiles have
+            if (n == 0) continue;
+            const int32_t vis = visible(p, t * a.tile_tokens + my_token);
             const int32_t tile_first = visible(p, t * a.tile_tokens);
             float top = -INFINITY, sum = 0.0f;   // top: the reference that weights are taken against, in score units
             for (uint32_t j = n; j-- > 0;) {
@@ -481,31 +566,56 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     break;
                 }
                 s_phase ^= 1u;
+                // The two tiles' softmaxes take turns, block by block: alone on the SM's units one is done twice as fast, and
+                // the other one's products run meanwhile.  Left to themselves they fall into step.
+                const bool turns = j < both;
+                if (turns) {
+                    if (!AT_WAIT(&bars->turn[t], turn_phase, 45)) {
+                        ok = false;
+                        break;
+                    }
+                    turn_phase ^= 1u;
+                }
                 __syncwarp();
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i += 1) tmem_ld32(s_at + i * 32u, s[i]);
-                tmem_ld_wait();
                 if ((int32_t)((j + 1u) * BLOCK_KEYS) > tile_first) {
+                    // some rows do not see all of the block: what they do not see becomes -infinity where it lies, so that the code
+                    // below, which every block runs, is short (straight through once a block, it is bound by its own fetching)
                     const int32_t seen = vis - (int32_t)(j * BLOCK_KEYS);   // columns below it are visible
+#pragma unroll 1
+                    for (int32_t i = 0; i < 4; i += 1) {
+                        if (__all_sync(0xffffffffu, seen >= i * 32 + 32)) continue;
+                        uint32_t s[32];
+                        tmem_ld32(s_at + (uint32_t)i * 32u, s);
+                        tmem_ld_wait32(s);
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i += 1) {
+                        for (int32_t e = 0; e < 32; e += 1) {
+                            if (e >= seen - i * 32) s[e] = 0xff800000u;
+                        }
+                        tmem_st32(s_at + (uint32_t)i * 32u, s);
+                    }
+                    tmem_st_wait();
+                }
+                // Scores are read twice, 32 columns at a time and each piece while the one before it is worked on: a whole row in
+                // registers would cost the other warps theirs.
+                uint32_t s[2][32];
+                float m[2] = {-INFINITY, -INFINITY};
+                tmem_ld32(s_at, s[0]);
+#pragma unroll 1
+                for (uint32_t half = 0; half < 2; half += 1) {
 #pragma unroll
-                        for (uint32_t e = 0; e < 32; e += 1) {
-                            if ((int32_t)(i * 32u + e) >= seen) s[i][e] = 0xff800000u;
+                    for (uint32_t i = 0; i < 2; i += 1) {
+                        tmem_ld_wait32(s[i]);
+                        tmem_ld32(s_at + ((half * 64u + i * 32u + 32u) & 127u), s[i ^ 1u]);   // behind the last piece the first again
+#pragma unroll
+                        for (uint32_t e = 0; e < 32; e += 4) {
+                            m[0] = max_nan(m[0], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                            m[1] = max_nan(m[1], __uint_as_float(s[i][e + 2]), __uint_as_float(s[i][e + 3]));
                         }
                     }
                 }
-                float m[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i += 1) {
-                    m[i] = __uint_as_float(s[i][0]);
-#pragma unroll
-                    for (uint32_t e = 1; e < 32; e += 1) m[i] = fmaxf(m[i], __uint_as_float(s[i][e]));
-                }
-                const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                const bool grows = (now - top) * to_log2 > GROW;   // also from -infinity; not from there to there
+                const float now = max_nan(m[0], m[1]);
+                const bool grows = now != -INFINITY && !((now - top) * to_log2 <= GROW);   // also from -infinity, and to NaN
                 if (j + 1u == n) {
                     top = now;
                 } else if (__any_sync(0xffffffffu, grows)) {
@@ -513,70 +623,117 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     const float f = grows ? exp2_fast((top - now) * to_log2) : 1.0f;
                     if (grows) top = now;
                     sum *= f;
-#pragma unroll
-                    for (uint32_t i = 0; i < HD / 32u; i += 1) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + i * 32u, o);
+                    tmem_ld_wait();
+#pragma unroll 1
+                    for (uint32_t i = 0; i < HD / 16u; i += 1) {
+                        uint32_t o[16];
+                        tmem_ld16(o_at + i * 16u, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (uint32_t e = 0; e < 32; e += 1) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(o_at + i * 32u, o);
+                        for (uint32_t e = 0; e < 16; e += 1) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st16(o_at + i * 16u, o);
                     }
                 }
-                const float base = top == -INFINITY ? 0.0f : SHIFT - top * to_log2;
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // against -infinity everything is -infinity: weights 0; against infinity or NaN everything is NaN
+                const float base = top == -INFINITY ? 0.0f : SHIFT - top * to_log2 + (top - top);
+                const uint64_t base2 = two(base, base);
+                uint64_t part[2] = {0, 0};
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i += 1) {
+                    tmem_ld_wait32(s[i & 1u]);
+                    if (i < 3) tmem_ld32(s_at + (i + 1u) * 32u, s[(i + 1u) & 1u]);
                     uint32_t w[16];
 #pragma unroll
                     for (uint32_t e = 0; e < 16; e += 1) {
-                        const float x = exp2_fast(fmaf(__uint_as_float(s[i][2 * e]), to_log2, base));
-                        const float y = exp2_fast(fmaf(__uint_as_float(s[i][2 * e + 1]), to_log2, base));
-                        part[e & 3u] += x + y;
+                        const uint64_t z = fma2(two(__uint_as_float(s[i & 1u][2 * e]), __uint_as_float(s[i & 1u][2 * e + 1])), scale2, base2);
+                        float x, y;
+                        if (e % POLY_OF < POLY_SHARE) {
+                            exp2_poly(z, x, y);
+                        } else {
+                            apart(z, x, y);
+                            x = exp2_fast(x);
+                            y = exp2_fast(y);
+                        }
+                        part[e & 1u] = add2(part[e & 1u], two(x, y));
                         // weights round to fp16 for the product (11 bits, as many as the output has); their sum does not
                         w[e] = pack_h2(x, y);
                     }
+                    if (i == 2 && turns && lane == 0) mbar_arrive(smem_u32(&bars->turn[t ^ 1u]));
                     tmem_st16(s_at + i * 16u, w);
+                    if ((i & 1u) != 0) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(smem_u32(&bars->p_full[t][i / 2u]));
+                    }
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(smem_u32(&bars->p_full[t]));
+                float x, y;
+                apart(add2(part[0], part[1]), x, y);
+                sum += x + y;
             }
-            if (!ok || !AT_WAIT(&bars->o_full[t], o_phase, 41)) break;
-            o_phase ^= 1u;
-            __syncwarp();
-            tc_fence_after();
-            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const bool extra = *(volatile uint32_t *)&bars->found[flag] != 0;
-            for (uint32_t i = 0; i < HD / 32u; i += 1) {
-                uint32_t o[32];
-                tmem_ld32(o_at + i * 32u, o);
-                tmem_ld_wait();
-                if (mine) {
-                    float y[32];
+            if (!ok || !AT_WAIT(&bars->sum_empty[t], sum_phase, 41)) break;
+            sum_phase ^= 1u;
+            bars->sum[t][row] = sum;
+            mbar_arrive(smem_u32(&bars->sum_full[t]));
+        }
+    } else {
+        // ---------------- output: a row per thread ----------------
+        const uint32_t row = (warp & 3u) * 32u + lane, my_token = row / a.group, my_head = row - my_token * a.group;
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16;
+        const bool whole = ((uintptr_t)a.o & 31u) == 0 && a.o_stride % 16u == 0;
+        uint32_t phase[2] = {0, 0}, n_item = 0;
+        bool ok = true;
+        while (ok && items.next(a, p, head)) {
+            const Blocks b = blocks_of(p, a.tile_tokens);
+            const uint32_t flag = n_item % FLAGS;
+            if (b.n != 0) n_item += 1;
 #pragma unroll
-                    for (uint32_t e = 0; e < 32; e += 1) y[e] = sum == 0.0f ? 0.0f : __uint_as_float(o[e]) * f;
-                    if (extra) {
-                        for (int32_t key = b.masked_from * (int32_t)BLOCK_KEYS; key < vis; key += 1) {
-                            const __half *v = a.v + (size_t)(p.k_row + (uint32_t)key) * a.kv_stride + (size_t)head * HD + i * 32u;
+            for (uint32_t t = 0; t < 2; t += 1) {
+                const uint32_t token = t * a.tile_tokens + my_token;   // behind the pair's first
+                const bool mine = my_token < a.tile_tokens && token < p.left;
+                __half *out = a.o + (size_t)(p.q_row + token) * a.o_stride + (size_t)(head * a.group + my_head) * HD;
+                if (b.tile[t] == 0) {   // no query, or none that sees a key
+                    if (mine) {
 #pragma unroll
-                            for (uint32_t e = 0; e < 32; e += 1) {
-                                const float x = __half2float(v[e]);
-                                if (!isfinite(x)) y[e] += x;
+                        for (uint32_t i = 0; i < HD; i += 8) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
+                    }
+                    continue;
+                }
+                ok = ok && AT_WAIT(&bars->sum_full[t], phase[t], 43) && AT_WAIT(&bars->o_full[t], phase[t], 44);
+                if (!ok) break;
+                phase[t] ^= 1u;
+                __syncwarp();
+                tc_fence_after();
+                const float sum = bars->sum[t][row];
+                mbar_arrive(smem_u32(&bars->sum_empty[t]));
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const bool extra = *(volatile uint32_t *)&bars->found[flag] != 0;
+                const int32_t vis = visible(p, token);
+#pragma unroll 1
+                for (uint32_t i = 0; i < HD / 16u; i += 1) {
+                    uint32_t o[16];
+                    tmem_ld16(tmem + 256u + t * HD + lanes + i * 16u, o);
+                    tmem_ld_wait();
+                    if (mine) {
+                        if (extra) {
+                            for (int32_t key = b.masked_from * (int32_t)BLOCK_KEYS; key < vis; key += 1) {
+                                const __half *v = a.v + (size_t)(p.k_row + (uint32_t)key) * a.kv_stride + (size_t)head * HD + i * 16u;
+#pragma unroll
+                                for (uint32_t e = 0; e < 16; e += 1) {
+                                    const float x = __half2float(v[e]);
+                                    if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                                }
                             }
                         }
-                    }
+                        uint32_t w[8];
 #pragma unroll
-                    for (uint32_t e = 0; e < 32; e += 8) {
-                        *reinterpret_cast<uint4 *>(out + i * 32u + e) =
-                            make_uint4(pack_h2(y[e], y[e + 1]), pack_h2(y[e + 2], y[e + 3]), pack_h2(y[e + 4], y[e + 5]), pack_h2(y[e + 6], y[e + 7]));
+                        for (uint32_t e = 0; e < 8; e += 1) w[e] = pack_h2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f);
+                        store32(out + i * 16u, w, whole);
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&bars->o_empty[t]));
             }
-            tc_fence_before();
-            mbar_arrive(smem_u32(&bars->o_empty[t]));
         }
     }
 #undef AT_WAIT
@@ -683,11 +840,11 @@ extern "C" void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k1
     const uint64_t pairs = (uint64_t)pc.rows_q / (2u * a.tile_tokens) + pc.seqs;   // at most
     MOE_REQUIRE(c, pairs * pc.kv_heads < (1ull << 31), "attn: too many tiles");
     CUtensorMap tq, tk, tv;
-    if (!moe_tmap_heads_f16(c, &tq, q16, pc.rows_q, pc.heads, pc.hd, pc.q_stride, a.group, a.tile_tokens)) return;
+    if (!moe_tmap_heads_f16(c, &tq, q16, pc.rows_q, pc.heads, pc.hd, pc.q_stride, a.group, a.tile_tokens, 1)) return;
     if (pc.rows_k == 0) {
         tk = tv = tq;   // never loaded from
-    } else if (!moe_tmap_heads_f16(c, &tk, k16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS) ||
-               !moe_tmap_heads_f16(c, &tv, v16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS)) {
+    } else if (!moe_tmap_heads_f16(c, &tk, k16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS, pc.hd / 64u) ||
+               !moe_tmap_heads_f16(c, &tv, v16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS, pc.hd / 64u)) {
         return;
     }
     moe_on_device on(c);

@@ -92,10 +92,10 @@ bool moe_tmap_tokens_f16(moe_cuda_ctx *c, moe_xmaps *out, const void *ptr, uint6
 // box (64 k, 2, 64 inter, 1 expert) lands in shared memory as 128 rows: row 2i = gate row i, row 2i+1 = up row i.
 bool moe_tmap_gate_up_f16(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint32_t experts, uint32_t inter, uint32_t k);
 
-// 3-D fp16 map over rows of heads (moe_attn.cu).
+// fp16 map over rows of heads (moe_attn.cu).
 bool moe_tmap_heads_f16(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint32_t rows, uint32_t heads, uint32_t hd, uint32_t stride,
-                        uint32_t box_heads, uint32_t box_rows);
-// 3-D map over the lines of a cache's rows (moe_decode.cu).
+                        uint32_t box_heads, uint32_t box_rows, uint32_t box_halves);
+// Map over the lines of a cache's rows (moe_decode.cu).
 bool moe_tmap_bytes(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint64_t rows, uint32_t row, uint32_t line, uint32_t box_rows);
 
 #define MOE_LIVE(c) ((c) != NULL && (c)->status == MOE_OK)

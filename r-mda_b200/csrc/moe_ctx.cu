@@ -397,13 +397,13 @@ bool moe_tmap_tokens_f16(moe_cuda_ctx *c, moe_xmaps *out, const void *ptr, uint6
     return true;
 }
 
-// Heads side by side in rows of `stride`: boxes of 64 columns, `box_heads` heads, `box_rows` rows, in shared memory row by
-// row and within a row head by head.
+// Heads side by side in rows of `stride`: boxes of `box_halves` times 64 columns of `box_heads` heads of `box_rows` rows.  In shared
+// memory the first 64 columns of all of them row by row and within a row head by head, then the next 64.
 bool moe_tmap_heads_f16(moe_cuda_ctx *c, CUtensorMap *out, const void *ptr, uint32_t rows, uint32_t heads, uint32_t hd, uint32_t stride,
-                        uint32_t box_heads, uint32_t box_rows) {
-    const cuuint64_t dims[3] = {hd, heads, rows}, strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
-    const cuuint32_t box[3] = {64, box_heads, box_rows};
-    return moe_encode(c, out, 3, ptr, dims, strides, box);
+                        uint32_t box_heads, uint32_t box_rows, uint32_t box_halves) {
+    const cuuint64_t dims[4] = {64, heads, rows, hd / 64}, strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2, 128};
+    const cuuint32_t box[4] = {64, box_heads, box_rows, box_halves};
+    return moe_encode(c, out, 4, ptr, dims, strides, box);
 }
 
 // Rows of `row` bytes without gaps, cut into lines of 64 or 128 bytes: boxes of `box_rows` rows, in shared memory line by line
