@@ -92,7 +92,7 @@ static inline const char *moe_attn_decode_refusal(const moe_cuda_kv_t *kv, const
     if (why != NULL) return why;
     if (!moe_stride_ok(pc.q_stride, (uint64_t)pc.heads * kv->hd) || !moe_stride_ok(pc.o_stride, (uint64_t)pc.heads * kv->hd))
         return "attn_decode: strides are multiples of 8 and hold all heads";
-    if (pc.seqs >= (1u << 20) || (uint64_t)pc.seqs * pc.heads >= (1ull << 31)) return "attn_decode: seqs below 2^20, seqs * heads below 2^31";
+    if (pc.seqs >= (1u << 20)) return "attn_decode: seqs below 2^20";
     if ((uint64_t)pc.table_stride * kv->page < pc.max_len || pc.max_len >= (1u << 31)) return "attn_decode: max_len needs more pages than a row of the table has";
     if (!(pc.scale > 0.0f && pc.scale <= 1.0e4f)) return "attn_decode: scale is positive, 10^4 at most";
     if (pc.seqs != 0 && (!moe_at16(q16) || !moe_at16(o16) || !moe_at4(len) || (pc.max_len != 0 && !moe_at4(table))))

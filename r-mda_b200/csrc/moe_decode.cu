@@ -1,12 +1,13 @@
 // Attention of one new token per sequence over the paged key-value cache.
 //
 // Bound by HBM: every cached key and value is read once, and a group of g query heads does 2 g operations per fp16 element.
-// The work is a line: sequence by sequence, head by head, stages of 16 or 32 cached tokens.  Every warp of a full chip takes an
-// equal piece of the line whatever the lengths are, so no SM waits for another, and walks it alone: its loads (TMA boxes of
-// one page's tokens, swizzled) run through a ring in shared memory that only it uses, with barriers that only it waits at,
-// and keep running across the ends of heads and sequences.  A (sequence, head) that lies within one warp's piece is written
-// out at once; the others leave their running maximum, sum and unnormalised output in the context's work area, and a second
-// small kernel joins them in the line's order.
+// The work is a line: sequence by sequence, head by head, stages of 16 or 32 cached tokens.  Every SM takes an equal piece of
+// the line whatever the lengths are, and every warp an equal piece of that, so no one waits for another.  A warp walks its
+// piece alone: its loads (TMA boxes of one page's tokens, swizzled) run through a ring in shared memory that only it uses, with
+// barriers that only it waits at, and keep running across the ends of heads and sequences.  A (sequence, head) that lies within
+// one warp's piece is written out at once; of the others each warp leaves its running maximum, sum and unnormalised output in
+// shared memory, the SM's warps join them, and heads that reach over an SM's piece go through the context's work area to a
+// second small kernel.  Everything is joined in the line's order.
 //
 // Scores are computed as S^T = K Q^T (16 tokens x 8 heads x 16 columns per mma.sync) and outputs as O^T = V^T P^T, so groups
 // of up to 8 heads waste nothing; P^T comes from S^T's accumulators by an 8x8 transpose (movmatrix).  Operands come from shared
@@ -28,11 +29,10 @@ struct DecArgs {
     const __half *q;
     const uint32_t *table, *len;
     __half *o;
-    unsigned long long *base;  // [seqs + 1]: stages of all sequences before s, of one head
-    float *part;               // [2 * warps][part_floats: g * hd outputs, g maxima, g sums]
+    uint4 *split;              // [SMs]: the head that begins in this SM's piece and goes on in others: sequence, kv head, first SM, SMs; 0 SMs: none
+    float *part;               // [2 * SMs][part_floats: g * hd outputs, g maxima, g sums]: of a head begun earlier, of one that goes on
     uint32_t pages, page, page_shift, kv_heads, group;
     uint32_t seqs, max_len, table_stride, q_stride, o_stride;
-    uint32_t warps;            // of the grid; part of the line that each takes follows from it and the line's length
     float scale;
     uint32_t *status;
     uint64_t wait_ns;
@@ -83,7 +83,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // Sizes of one stage of one warp's ring, and how many warps share an SM.
 template <uint32_t HD, uint32_t NT, bool FP8>
 struct Stage {
-    static constexpr uint32_t WARPS = NT == 2 ? 8 : 12;
+    static constexpr uint32_t WARPS = 8;
     static constexpr uint32_t THREADS = WARPS * 32;
     static constexpr uint32_t ROW = HD * (FP8 ? 1 : 2);             // bytes of a token's keys, or values
     static constexpr uint32_t LINE = ROW > 128 ? 128 : ROW;         // of them in one swizzled line; two halves if ROW is 256
@@ -94,10 +94,12 @@ struct Stage {
     static constexpr uint32_t K_BYTES = TOKENS * ROW;
     static constexpr uint32_t BYTES = 2 * K_BYTES;
     static constexpr uint32_t SCALES = FP8 ? 2 * TOKENS * 4 : 0;    // keys' scales, then values'
-    static constexpr uint32_t ROOM = 212000 / WARPS / (BYTES + SCALES);
+    static constexpr uint32_t PART = (8 * NT * (HD + 2) * 4 + 15) / 16 * 16;   // a part of a head, for the largest group
+    static constexpr uint32_t ROOM = (218000 / WARPS - PART) / (BYTES + SCALES);
     static constexpr uint32_t COUNT = ROOM > 4 ? 4 : ROOM;
     static constexpr uint32_t RING = WARPS * COUNT * BYTES;
-    static constexpr uint32_t SMEM = RING + WARPS * COUNT * SCALES + WARPS * COUNT * 8 + 1024;
+    static constexpr uint32_t PARTS = (RING + WARPS * COUNT * (SCALES + 8) + 15) / 16 * 16;   // where the parts of heads lie
+    static constexpr uint32_t SMEM = PARTS + WARPS * PART + 1024;
 };
 
 // A place on the line: stage `g` of head h of sequence s.
@@ -138,9 +140,13 @@ __device__ __forceinline__ bool landed(uint32_t bar, uint32_t parity, const DecA
     return __all_sync(0xffffffffu, ok);
 }
 
-// Where the j-th of `warps` pieces of a line of `total` stages begins.
-__device__ __forceinline__ unsigned long long piece_begin(unsigned long long total, uint32_t j, uint32_t warps) {
-    return total * j / warps;
+// x * j / n, in 32 bits where they do (64-bit division takes hundreds of cycles).
+__device__ __forceinline__ unsigned long long share_of(unsigned long long x, uint32_t j, uint32_t n) {
+    return x < (1u << 22) ? (unsigned long long)((uint32_t)x * j / n) : x * j / n;   // j up to 2^10
+}
+// The last j with total * j / n <= x: the piece of n that holds stage x.
+__device__ __forceinline__ uint32_t piece_of(unsigned long long x, unsigned long long total, uint32_t n) {
+    return total < (1u << 22) ? (((uint32_t)x + 1u) * n - 1u) / (uint32_t)total : (uint32_t)(((x + 1u) * n - 1u) / total);
 }
 
 template <uint32_t HD, uint32_t NT, bool FP8>
@@ -157,6 +163,13 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     uint8_t *const my_ring = smem + warp * St::COUNT * St::BYTES;
     const uint32_t ring0 = smem_u32(my_ring), scales0 = smem_u32(smem) + St::RING + warp * St::COUNT * St::SCALES;
     const uint32_t bars0 = smem_u32(smem) + St::RING + DEC_WARPS * St::COUNT * St::SCALES + warp * St::COUNT * 8u;
+    // parts of heads: a warp's first one, which begins before it, and its last one, which goes on behind it (in its ring, at the end)
+    float *const ended = reinterpret_cast<float *>(smem + St::PARTS);
+    auto goes_on = [&](uint32_t w) { return reinterpret_cast<float *>(smem + w * St::COUNT * St::BYTES); };
+    __shared__ uint2 ended_of[DEC_WARPS], goes_on_of[DEC_WARPS];   // sequence and kv head; a sequence of ~0: none
+    __shared__ bool begins[DEC_WARPS];   // the last one begins in the warp's piece
+    __shared__ uint32_t behind;          // stages of the SM's last head behind its piece
+    __shared__ uint4 over;               // the head that begins in the SM's piece and goes on behind it: sequence, kv head, first SM, SMs
     if (lane < St::COUNT) {
         mbar_init(bars0 + lane * 8u, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -181,22 +194,25 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     for (uint32_t w = 0; w < DEC_WARPS; w += 1) first += w < warp ? warp_sum[w] : 0ull;
     before[threadIdx.x] = first;
     if (threadIdx.x == DEC_THREADS - 1u) before[DEC_THREADS] = first + mine;
-    if (blockIdx.x == 0) {  // for the joining kernel
-        unsigned long long at = first;
-        for (uint32_t s = s_lo; s < s_hi; s += 1) {
-            a.base[s] = at;
-            at += stages_of(a, s, PER);
-            if (a.len[s] > a.max_len) moe_deny(a.status, MOE_SITE_LENGTH);
-        }
-        if (threadIdx.x == DEC_THREADS - 1u) a.base[a.seqs] = first + mine;
-    }
     __syncthreads();
     const unsigned long long total = before[DEC_THREADS] * a.kv_heads;
-    const uint32_t warps = total < a.warps ? (uint32_t)total : a.warps;
-    const uint32_t me = warp * gridDim.x + blockIdx.x;  // neighbours on the line run on different SMs
-    if (me >= warps) return;
-    const unsigned long long x0 = piece_begin(total, me, warps);
-    uint32_t left = (uint32_t)(piece_begin(total, me + 1u, warps) - x0);
+    // SMs in use: as many as leave every warp at least a stage
+    const uint32_t sms = (uint32_t)min((unsigned long long)gridDim.x, (total + DEC_WARPS - 1u) / DEC_WARPS);
+    for (uint32_t s = warp * gridDim.x + blockIdx.x; s < a.seqs; s += DEC_WARPS * gridDim.x) {   // nothing to attend to: zeros
+        if (stages_of(a, s, PER) != 0u) continue;
+        __half *out = a.o + (size_t)s * a.o_stride;
+        for (uint32_t i = lane * 8u; i < a.kv_heads * a.group * HD; i += 256u) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
+    }
+    if (blockIdx.x >= sms) {
+        if (threadIdx.x == 0) a.split[blockIdx.x] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const unsigned long long sm0 = share_of(total, blockIdx.x, sms), sm1 = share_of(total, blockIdx.x + 1u, sms);
+    const uint32_t warps = (uint32_t)min((unsigned long long)DEC_WARPS, sm1 - sm0);
+    if (lane == 0) ended_of[warp] = goes_on_of[warp] = make_uint2(~0u, 0u);
+    // a warp without a piece waits for the others at the first one's beginning
+    const unsigned long long x0 = sm0 + (warp < warps ? share_of(sm1 - sm0, warp, warps) : 0ull);
+    uint32_t left = warp < warps ? (uint32_t)(sm0 + share_of(sm1 - sm0, warp + 1u, warps) - x0) : 0u;
 
     // ---- its beginning -----------------------------------------------------------------------------
     uint32_t owner = 0;  // the last thread share that begins at or before x0 (and is not empty)
@@ -216,11 +232,14 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             p.s += 1;
             p.stages = stages_of(a, p.s, PER);
         }
-        p.h = (uint32_t)((x0 - at) / p.stages);
-        p.g = (uint32_t)(x0 - at - (unsigned long long)p.h * p.stages);
+        const unsigned long long off = x0 - at;   // below stages * kv heads
+        p.h = off < (1ull << 32) ? (uint32_t)off / p.stages : (uint32_t)(off / p.stages);
+        p.g = (uint32_t)(off - (unsigned long long)p.h * p.stages);
         p.len = a.len[p.s];
     }
 
+    if (threadIdx.x == 0) over = make_uint4(0, 0, 0, 0);
+    auto sm_of = [&](unsigned long long x) { return piece_of(x, total, sms); };
     Place q = p;             // the next stage to load, and the pages of its boxes
     uint32_t to_load = left, pg[SG];
     const uint32_t box = a.page < PER ? a.page : PER;   // tokens of one box: a stage, or a page of 16 of a stage of 32
@@ -476,9 +495,10 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             phase ^= 1u;
         }
         const bool head_ends = p.g + 1u == p.stages;
+        bool whole_head = false;
         if (head_ends || left == 0) {
             fresh = true;
-            const bool whole = head_ends && begun_at == 0;
+            whole_head = head_ends && begun_at == 0;
 #pragma unroll
             for (uint32_t n = 0; n < NT; n += 1) {
                 float l[2];
@@ -489,7 +509,7 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
                     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
                 }
-                if (whole) {
+                if (whole_head) {
                     // transposed back, a lane has two neighbouring columns of head r; of e4m3 the tile's rows 8-15 are its odd columns
                     const float f0 = l[0] == 0.0f ? 0.0f : 1.0f / l[0], f1 = l[1] == 0.0f ? 0.0f : 1.0f / l[1];
                     const uint32_t head = n * 8u + r;
@@ -506,8 +526,7 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                         }
                     }
                 } else {
-                    // place 0: the piece began inside this head; place 1: the head goes on in the next warp's piece
-                    float *part = a.part + (size_t)(me * 2u + (begun_at == 0 ? 1u : 0u)) * part_floats(a.group, HD);
+                    float *part = head_ends ? ended + warp * (St::PART / 4u) : goes_on(warp);
 #pragma unroll
                     for (uint32_t e = 0; e < 2; e += 1) {
                         const uint32_t head = n * 8u + 2u * c + e;
@@ -525,6 +544,15 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                 }
             }
         }
+        if (fresh && !whole_head && lane == 0) {
+            if (head_ends) {
+                ended_of[warp] = make_uint2(p.s, p.h);
+            } else {
+                goes_on_of[warp] = make_uint2(p.s, p.h);
+                begins[warp] = begun_at == 0;
+                if (warp + 1u == warps) behind = p.stages - p.g - 1u;
+            }
+        }
         if (left != 0) place_next(a, p, PER);
     }
     if (FP8) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -535,44 +563,102 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             if (done) break;
         }
     }
+
+    // ---- heads that go on from one warp to the next ------------------------------------------------
+    __syncthreads();
+    float *const begun_earlier = a.part + (size_t)blockIdx.x * 2u * part_floats(a.group, HD);
+    const uint32_t at_top = a.group * HD, at_sum = a.group * (HD + 1u);
+    // lane w looks at warp w: whether its last head goes on, and is one that an earlier warp has told of
+    const uint2 key_of = lane < warps ? goes_on_of[lane] : make_uint2(~0u, 0u), key_before = lane != 0 && lane < warps ? goes_on_of[lane - 1u] : make_uint2(~0u, 0u);
+    const uint2 end_of = lane < warps ? ended_of[lane] : make_uint2(~0u, 0u);
+    const bool here_of = lane < warps && begins[lane];
+    const uint32_t goes = __ballot_sync(0xffffffffu, key_of.x != ~0u), heres = __ballot_sync(0xffffffffu, here_of);
+    const uint32_t starts = goes & __ballot_sync(0xffffffffu, here_of || key_of.x != key_before.x || key_of.y != key_before.y);
+    for (uint32_t todo = starts; todo != 0u; todo &= todo - 1u) {
+        const uint32_t w0 = (uint32_t)__ffs((int)todo) - 1u;
+        const uint32_t stop = (~goes | starts) & (0xfffffffeu << w0);   // the first warp behind w0 whose last head is another
+        const uint32_t w1 = stop != 0u ? min((uint32_t)__ffs((int)stop) - 1u, warps) : warps;
+        const uint2 key = make_uint2(__shfl_sync(0xffffffffu, key_of.x, w0), __shfl_sync(0xffffffffu, key_of.y, w0));
+        const uint32_t end_s = __shfl_sync(0xffffffffu, end_of.x, w1 & 31u), end_h = __shfl_sync(0xffffffffu, end_of.y, w1 & 31u);
+        const bool ends = w1 < warps && end_s == key.x && end_h == key.y, here = (heres >> w0 & 1u) != 0u;
+        const uint32_t n = w1 - w0 + (ends ? 1u : 0u);
+        for (uint32_t head = warp; head < a.group; head += DEC_WARPS) {
+            // lane i: the i-th part's maximum and sum
+            const float *mine = lane < w1 - w0 ? goes_on(w0 + lane) : ended + (w1 < warps ? w1 : 0u) * (St::PART / 4u);
+            float m = lane < n ? mine[at_top + head] : -INFINITY;
+            const float own = m;
+#pragma unroll
+            for (uint32_t o = 16; o != 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float f_of = lane >= n ? 0.0f : own == m ? 1.0f : exp2_fast(own - m);
+            float sum = lane < n ? f_of * mine[at_sum + head] : 0.0f;
+#pragma unroll
+            for (uint32_t o = 16; o != 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t i = 0; i < DEC_WARPS + 1u; i += 1) {
+                if (i >= n) break;
+                const float *part = i < w1 - w0 ? goes_on(w0 + i) : ended + w1 * (St::PART / 4u);
+                const float f = __shfl_sync(0xffffffffu, f_of, i);
+                const float4 v = *reinterpret_cast<const float4 *>(part + head * HD + (lane < HD / 4u ? lane * 4u : 0u));
+                y.x += f * v.x;
+                y.y += f * v.y;
+                y.z += f * v.z;
+                y.w += f * v.w;
+            }
+            if (lane >= HD / 4u) continue;
+            if (here && ends) {
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                __half *out = a.o + (size_t)key.x * a.o_stride + (size_t)(key.y * a.group + head) * HD;
+                *reinterpret_cast<uint2 *>(out + lane * 4u) = make_uint2(pack_h2(y.x * f, y.y * f), pack_h2(y.z * f, y.w * f));
+            } else {
+                float *to = begun_earlier + (here ? part_floats(a.group, HD) : 0u);
+                *reinterpret_cast<float4 *>(to + head * HD + lane * 4u) = y;
+                if (lane == 0) {
+                    to[at_top + head] = m;
+                    to[at_sum + head] = sum;
+                }
+            }
+        }
+        if (here && !ends && threadIdx.x == 0) over = make_uint4(key.x, key.y, blockIdx.x, sm_of(sm1 + behind - 1u) - blockIdx.x + 1u);
+    }
+    if (ended_of[0].x != ~0u) {   // begun in an earlier SM's piece, ended in this one's first warp
+        for (uint32_t i = threadIdx.x; i < a.group * (HD + 2u); i += DEC_THREADS) begun_earlier[i] = ended[i];
+    }
+
+    if (blockIdx.x == 0) {
+        for (uint32_t s = s_lo; s < s_hi; s += 1) {
+            if (a.len[s] > a.max_len) moe_deny(a.status, MOE_SITE_LENGTH);
+        }
+    }
+    if (threadIdx.x == 0) a.split[blockIdx.x] = over;
 }
 
-// One block per (sequence, query head): joins the pieces of a head that several warps worked on -- each warp of the block every
-// eighth piece, then the warps' sums, always in the line's order -- and writes zeros for an empty sequence.
-constexpr uint32_t JOIN_WARPS = 8;
+// Joins a head that begins in one SM's piece and goes on in others: a block for each SM and query head of a group, a warp for every
+// fourth piece, always in the line's order.
+constexpr uint32_t JOIN_WARPS = 4;
 template <uint32_t HD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) moe_attn_join_kernel(DecArgs a) {
     __shared__ float4 y_of[JOIN_WARPS][HD / 4];
     __shared__ float sum_of[JOIN_WARPS];
     moe_pdl_begin();
-    const uint32_t heads = a.kv_heads * a.group, s = blockIdx.x / heads, qh = blockIdx.x - s * heads, h = qh / a.group, head = qh - h * a.group;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const unsigned long long b0 = a.base[s], stages = a.base[s + 1u] - b0;
-    __half *out = a.o + (size_t)s * a.o_stride + (size_t)qh * HD;
-    if (stages == 0) {
-        if (threadIdx.x < HD / 4u) *reinterpret_cast<uint2 *>(out + threadIdx.x * 4u) = make_uint2(0, 0);
-        return;
-    }
-    const unsigned long long total = a.base[a.seqs] * a.kv_heads, x0 = b0 * a.kv_heads + h * stages, x1 = x0 + stages;
-    const uint32_t warps = total < a.warps ? (uint32_t)total : a.warps;
-    // the piece that holds x: the largest j with total * j / warps <= x
-    const uint32_t w0 = (uint32_t)(((x0 + 1u) * warps - 1u) / total), w1 = (uint32_t)((x1 * warps - 1u) / total);
-    if (w0 == w1) return;
-    const uint32_t size = part_floats(a.group, HD), n = w1 - w0 + 1u;
-    auto piece = [&](uint32_t i) { return a.part + (size_t)((w0 + i) * 2u + (i == 0 ? 1u : 0u)) * size; };
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32u) top = fmaxf(top, piece(i)[a.group * HD + head]);
+    const uint32_t first = blockIdx.x / a.group, head = blockIdx.x - first * a.group;
+    const uint4 split = a.split[first];   // sequence, kv head, first SM, SMs
+    if (split.w == 0u) return;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, size = part_floats(a.group, HD), n = split.w;
+    auto part_at = [&](uint32_t i) { return a.part + (size_t)((first + i) * 2u + (i == 0 ? 1u : 0u)) * size; };
+    const uint32_t at_top = a.group * HD + head, at_sum = a.group * (HD + 1u) + head;
+    float m = -INFINITY, sum = 0.0f;
+    for (uint32_t i = lane; i < n; i += 32u) m = fmaxf(m, part_at(i)[at_top]);
 #pragma unroll
-    for (uint32_t o = 16; o != 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f;
+    for (uint32_t o = 16; o != 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const bool mine = lane < HD / 4u;
 #pragma unroll 4
     for (uint32_t i = warp; i < n; i += JOIN_WARPS) {
-        const float *part = piece(i);
-        const float m = part[a.group * HD + head], l = part[a.group * (HD + 1u) + head];
+        const float *part = part_at(i);
+        const float top = part[at_top], l = part[at_sum];
         const float4 v = *reinterpret_cast<const float4 *>(part + head * HD + (mine ? lane * 4u : 0u));
-        const float f = m == top ? 1.0f : exp2_fast(m - top);
+        const float f = top == m ? 1.0f : exp2_fast(top - m);
         sum += f * l;
         y.x += f * v.x;
         y.y += f * v.y;
@@ -595,27 +681,26 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) moe_attn_join_kernel(DecArgs 
         y.w += v.w;
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    __half *out = a.o + (size_t)split.x * a.o_stride + (size_t)(split.y * a.group + head) * HD;
     *reinterpret_cast<uint2 *>(out + threadIdx.x * 4u) = make_uint2(pack_h2(y.x * f, y.y * f), pack_h2(y.z * f, y.w * f));
 }
 
 template <uint32_t HD, uint32_t NT, bool FP8>
-void decode_launch(moe_cuda_ctx *c, const moe_cuda_kv_t *kv, const DecArgs &args, uint32_t slot) {
+void decode_launch(moe_cuda_ctx *c, const moe_cuda_kv_t *kv, const DecArgs &a, uint32_t slot) {
     using St = Stage<HD, NT, FP8>;
     constexpr uint32_t smem = St::SMEM;
-    static_assert(St::COUNT >= 2 && St::COUNT * St::SG <= 32 && smem + 8192 <= 227 * 1024, "ring");
+    static_assert(St::COUNT >= 2 && St::COUNT * St::SG <= 32 && smem + 4096 <= 227 * 1024 && St::PART <= St::COUNT * St::BYTES, "ring");
     CUtensorMap tk, tv;
     const uint64_t rows = (uint64_t)kv->pages * kv->kv_heads * kv->page;
     const uint32_t box = kv->page < St::TOKENS ? kv->page : St::TOKENS;
     if (!moe_tmap_bytes(c, &tk, kv->k, rows, St::ROW, St::LINE, box) || !moe_tmap_bytes(c, &tv, kv->v, rows, St::ROW, St::LINE, box)) return;
-    DecArgs a = args;
-    a.warps = (uint32_t)c->sm_count * St::WARPS;
     if (!c->dec_attr_set[slot]) {
         MOE_CUDA_TRY(c, cudaFuncSetAttribute(moe_attn_decode_kernel<HD, NT, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         c->dec_attr_set[slot] = true;
     }
     moe_run(c, moe_attn_decode_kernel<HD, NT, FP8>, (uint32_t)c->sm_count, St::THREADS, smem, tk, tv, a);
     MOE_LAUNCHED(c);
-    moe_run(c, moe_attn_join_kernel<HD>, a.seqs * a.kv_heads * a.group, JOIN_WARPS * 32, 0, a);
+    moe_run(c, moe_attn_join_kernel<HD>, (uint32_t)c->sm_count * a.group, JOIN_WARPS * 32, 0, a);
     MOE_LAUNCHED(c);
 }
 
@@ -644,18 +729,17 @@ extern "C" void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv,
     a.table_stride = pc.table_stride;
     a.q_stride = pc.q_stride;
     a.o_stride = pc.o_stride;
-    a.warps = (uint32_t)c->sm_count * 16u;   // at most; the variant sets its own
     a.scale = pc.scale;
     a.status = c->dev_status_dev;
     a.wait_ns = c->wait_ns;
-    const size_t base_bytes = (((size_t)pc.seqs + 1u) * 8u + 255u) & ~(size_t)255u;
-    const size_t part_bytes = (size_t)a.warps * 2u * part_floats(a.group, kv->hd) * 4u;
-    if (base_bytes + part_bytes > c->work_bytes) {
-        moe_fail(c, MOE_ERR_NOMEM, "attn_decode: %zu bytes of work area, the context has %zu", base_bytes + part_bytes, c->work_bytes);
+    const size_t split_bytes = (size_t)c->sm_count * sizeof(uint4);
+    const size_t part_bytes = split_bytes + (size_t)c->sm_count * 2u * part_floats(a.group, kv->hd) * 4u;
+    if (part_bytes > c->work_bytes) {
+        moe_fail(c, MOE_ERR_NOMEM, "attn_decode: %zu bytes of work area, the context has %zu", part_bytes, c->work_bytes);
         return;
     }
-    a.base = (unsigned long long *)c->work;
-    a.part = (float *)((uint8_t *)c->work + base_bytes);
+    a.split = (uint4 *)c->work;
+    a.part = (float *)((uint8_t *)c->work + split_bytes);
     moe_on_device on(c);
     const bool fp8 = kv->type == MOE_KV_E4M3, wide = a.group > 8u;
     if (kv->hd == 128u) {
