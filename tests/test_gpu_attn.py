@@ -1,5 +1,6 @@
 """The attention half of a layer against plain 64-bit forms: rotary positions, the paged key-value cache (fp16 and e4m3),
 attention over packed prompts and of one new token over the cache, alone and together."""
+import ctypes as C
 import math
 
 import numpy as np
@@ -402,3 +403,318 @@ def test_attn_several_items_to_every_sm_and_call_after_call(on, hd, heads, kv_he
             o, mass, size = R.attention(q[a + lo:a + hi].double(), k[b:b + n].double(), v[b:b + n].double(), hd ** -0.5, n - m + lo)
             R.check(outs[0][a + lo:a + hi], o, mass, size, hd, n)
         a, b = a + m, b + n
+
+
+# ---- refusals that only the device can see --------------------------------------------------------
+def _refused(mc, run, kind):
+    """run(context) on a context of its own: MOE_ERR_ARG by the next flush, and later calls do nothing."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = mc.Ctx(0, stream.cuda_stream)
+        c.check()
+        run(c)
+        with pytest.raises(mc.MoeCudaError, match=kind):
+            c.flush()
+        assert c.status() == mc.MOE_ERR_ARG
+        torch.cuda.synchronize()
+        c.close()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_slots_outside_the_cache(mc, e4m3):
+    g = _gen(1)
+    kv = Cache(mc, g, 3, 16, 2, 64, e4m3)
+    before = [t.clone() for t in (kv.k.view(torch.uint8), kv.v.view(torch.uint8))]
+    x = _f16(g, 4, 128)
+    slot = _u32([5, 48, 0x7FFFFFFF, NO_SLOT])
+
+    def run(c):
+        c.kv_write(kv.c, x.data_ptr(), x.data_ptr(), slot.data_ptr(), 4)
+
+    _refused(mc, run, "cache slot")
+    for t, b in zip((kv.k.view(torch.uint8), kv.v.view(torch.uint8)), before):   # slot 5 alone is written
+        same = (t == b).view(3, 2, 16, -1).all(-1).all(1)
+        same[0, 5] = True
+        assert same.all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pages_outside_the_cache(mc, e4m3, hd):
+    """Rows of bad pages are left, the others are read; a decode counts their tokens as not there."""
+    g = _gen(2)
+    kv = Cache(mc, g, 5, 16, 2, hd, e4m3)
+    table = torch.tensor([[0, 0x7FFFFFF0, 2], [3, 5, 4]], device="cuda", dtype=torch.int32)
+    cu, length = _u32([0, 48, 90]), _u32([48, 42])
+    k, v = (torch.full((90, 2 * hd), 7.0, device="cuda", dtype=torch.float16) for _ in range(2))
+    q, out = _f16(g, 2, 4 * hd), torch.full((2, 4 * hd), 7.0, device="cuda", dtype=torch.float16)
+
+    def read(c):
+        c.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), 2, 90, 3)
+
+    def decode(c):
+        c.attn_decode(kv.c, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), 2, 4, 48, 3)
+
+    _refused(mc, read, "page")
+    assert (k[16:32] == 7).all() and (v[64:80] == 7).all()
+    rk, _ = kv.rows(torch.tensor([0, 2], device="cuda"), 32)
+    assert torch.equal(k[:16].view(16, 2, hd), rk[:16].half()) and torch.equal(k[32:48].view(16, 2, hd), rk[16:].half())
+    _refused(mc, decode, "page")
+    for i, (pages, n) in enumerate((([0, 2], 32), ([3, 4], 26))):
+        x = kv.rows(torch.tensor(pages, device="cuda"), n)
+        o, mass, size = R.attention(q[i:i + 1].double().view(1, 4, hd), *x, hd ** -0.5, n - 1)
+        R.check(out[i:i + 1].view(1, 4, hd), o, mass, size, hd, n)
+
+
+def test_lengths_beyond_the_bound(mc):
+    g = _gen(3)
+    kv = Cache(mc, g, 4, 16, 1, 64, False)
+    table, length = torch.tensor([[0, 1], [2, 3]], device="cuda", dtype=torch.int32), _u32([0xFFFFFFFF, 20])
+    q, out = _f16(g, 2, 64), torch.full((2, 64), 7.0, device="cuda", dtype=torch.float16)
+    _refused(mc, lambda c: c.attn_decode(kv.c, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), 2, 1, 32, 2), "length")
+    assert (out[0] == 0).all()
+    x = kv.rows(table[1].long(), 20)
+    R.check(out[1:].view(1, 1, 64), *R.attention(q[1:].double().view(1, 1, 64), *x, 0.125, 19), 64, 20)
+
+
+@pytest.mark.parametrize("cu_q,cu_k", [([0, 9], [0, 40]), ([0, 300], [0, 40]), ([5, 2], [0, 40]), ([0, 9, 5], [0, 20, 40]), ([0, 5, 9], [0, 50, 40])])
+def test_row_ranges_outside_the_tensors(mc, cu_q, cu_k):
+    """Offsets that fall, or pass the tensors' rows, are refused without a read outside them (8 query rows, 40 key rows)."""
+    g = _gen(4)
+    q, k, out = _f16(g, 8, 64), _f16(g, 40, 64), torch.full((9, 64), 7.0, device="cuda", dtype=torch.float16)
+    a, b = _u32(cu_q), _u32(cu_k)
+    _refused(mc, lambda c: c.attn(q.data_ptr(), k.data_ptr(), k.data_ptr(), a.data_ptr(), b.data_ptr(), out.data_ptr(), len(cu_q) - 1, 8, 40, 1, 1, 64), "row range")
+    assert (out[8] == 7).all()
+
+
+def test_host_refusals_are_sticky(mc):
+    with mc.Ctx(0) as c:
+        c.check()
+        b = c.alloc(4096)
+        c.attn(b, b, b, b, b, b, 1, 4, 4, 3, 2, 64)
+        assert c.status() == mc.MOE_ERR_ARG and "query heads" in c.last_error()
+
+
+def test_nothing_to_do(on, mc):
+    """No rows, no sequences: no launch, no error."""
+    kv = Cache(mc, _gen(1), 1, 16, 1, 64, False)
+    n = on.launches()
+    on.rope(None, None, None, 0, 1, 1, 64, 64, 1e4)
+    on.kv_write(kv.c, None, None, None, 0)
+    on.kv_read(kv.c, None, None, None, None, 0, 0, 1)
+    on.attn(None, None, None, None, None, None, 0, 0, 0, 1, 1, 64)
+    on.attn_decode(kv.c, None, None, None, None, 0, 1, 0, 1)
+    on.flush()
+    assert on.launches() == n
+
+
+# ---- streams, graphs, contexts ----------------------------------------------------------------------
+def _run_of_calls(c, s):
+    """Rotary positions, cache, prompt attention, read-back and a decode step, one behind the other."""
+    h, g, hd, rows = 8, 2, 64, s["rows"]
+    cols = (h + 2 * g) * hd
+    c.rope(s["x"].data_ptr(), s["pos"].data_ptr(), s["p"].data_ptr(), rows, h + 2 * g, h + g, hd, hd, 1e4)
+    at = s["p"].data_ptr()
+    c.kv_write(s["kv"].c, at + 2 * h * hd, at + 2 * (h + g) * hd, s["slot"].data_ptr(), rows, cols)
+    c.attn(at, at + 2 * h * hd, at + 2 * (h + g) * hd, s["cu"].data_ptr(), s["cu"].data_ptr(), s["o"].data_ptr(), 2, rows, rows, h, g, hd, cols, cols)
+    c.kv_read(s["kv"].c, s["table"].data_ptr(), s["cu"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), 2, rows, s["table"].shape[1])
+    c.attn_decode(s["kv"].c, s["q"].data_ptr(), s["table"].data_ptr(), s["len"].data_ptr(), s["od"].data_ptr(), 2, h, max(s["lengths"]), s["table"].shape[1])
+
+
+def _calls_state(mc, seed, lengths):
+    gen = _gen(seed)
+    h, g, hd, page, rows = 8, 2, 64, 16, sum(lengths)
+    per = [-(-n // page) for n in lengths]
+    kv = Cache(mc, gen, sum(per), page, g, hd, True)
+    table = _table(gen, lengths, page, sum(per), max(per))
+    place = torch.cat([torch.arange(n, device="cuda") for n in lengths])
+    seq = torch.cat([torch.full((n,), i, device="cuda") for i, n in enumerate(lengths)])
+    slot = (table[seq, place // page] * page + place % page).int()
+    f = lambda *shape: torch.full(shape, 7.0, device="cuda", dtype=torch.float16)  # noqa: E731
+    return {"rows": rows, "lengths": lengths, "x": torch.randn(rows, (h + 2 * g) * hd, device="cuda", generator=gen), "pos": place.int(), "slot": slot,
+            "kv": kv, "table": table, "cu": _starts(lengths), "len": _u32(lengths), "q": _f16(gen, 2, h * hd), "p": f(rows, (h + 2 * g) * hd),
+            "o": f(rows, h * hd), "k": f(rows, g * hd), "v": f(rows, g * hd), "od": f(2, h * hd)}
+
+
+def test_run_together(on, mc):
+    """Each step against the plain form of what the step before it left."""
+    s = _calls_state(mc, 11, [75, 130])
+    _run_of_calls(on, s)
+    on.flush()
+    h, g, hd = 8, 2, 64
+    p = s["p"].view(-1, h + 2 * g, hd)
+    kd, vd = (R.e4m3(p[:, a:a + g]) for a in (h, h + g))
+    kd, vd = (c.double() * sc.double()[..., None] for c, sc in (kd, vd))
+    assert torch.equal(s["k"].view(-1, g, hd), kd.half()) and torch.equal(s["v"].view(-1, g, hd), vd.half())
+    at = 0
+    for i, n in enumerate(s["lengths"]):
+        q, k, v = (p[at:at + n, a:b].double() for a, b in ((0, h), (h, h + g), (h + g, h + 2 * g)))
+        R.check(s["o"][at:at + n].view(n, h, hd), *R.attention(q, k, v, 0.125, 0), hd, n)
+        R.check(s["od"][i:i + 1].view(1, h, hd), *R.attention(s["q"][i:i + 1].double().view(1, h, hd), kd[at:at + n], vd[at:at + n], 0.125, n - 1), hd, n)
+        at += n
+
+
+def test_captured_and_replayed(mc):
+    """One graph of all calls, replayed on new values in the same buffers; then a second graph of the same context."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = mc.Ctx(0, stream.cuda_stream)
+        c.check()
+        a, b = _calls_state(mc, 21, [75, 130]), _calls_state(mc, 22, [300, 1])
+        graphs = []
+        for s in (a, b):
+            _run_of_calls(c, s)   # kernels are loaded before a capture
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                _run_of_calls(c, s)
+            graphs.append(graph)
+        for s, graph, seed in ((a, graphs[0], 31), (b, graphs[1], 32), (a, graphs[0], 33)):
+            s["x"].copy_(torch.randn(s["x"].shape, device="cuda", generator=_gen(seed)))
+            for n in ("p", "o", "k", "v", "od"):
+                s[n].fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            got = {n: s[n].clone() for n in ("p", "o", "k", "v", "od")}
+            for n in got:
+                s[n].fill_(7.0)
+            _run_of_calls(c, s)
+            c.flush()
+            for n in got:
+                assert torch.equal(got[n], s[n]), n
+        del graphs
+        c.close()
+
+
+def test_two_contexts_at_once(mc):
+    """Two contexts on streams of their own, both at work: each has its own work area."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [mc.Ctx(0, s.cuda_stream) for s in streams]
+    states = [_calls_state(mc, 41 + i, n) for i, n in enumerate(([700, 900], [1500, 64]))]
+    torch.cuda.synchronize()
+    want = []
+    for c, s in zip(ctxs, states):
+        _run_of_calls(c, s)
+        c.flush()
+        want.append({n: s[n].clone() for n in ("o", "od", "k")})
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s in zip(ctxs, states):
+            _run_of_calls(c, s)
+    for c, s, w in zip(ctxs, states, want):
+        c.flush()
+        for n in w:
+            assert torch.equal(s[n], w[n]), n
+        c.close()
+
+
+def test_calls_allocate_nothing(on, mc):
+    s = _calls_state(mc, 51, [200, 77])
+    _run_of_calls(on, s)
+    on.flush()
+    free0, _ = torch.cuda.mem_get_info(0)
+    mc.lib().moe_cuda_fail_alloc_after(on.p, 1)
+    _run_of_calls(on, s)
+    on.flush()
+    assert torch.cuda.mem_get_info(0)[0] == free0
+
+
+# ---- the C host side ---------------------------------------------------------------------------------
+class Attn(C.Structure):
+    _fields_ = ([("c", C.c_void_p)] + [(n, C.c_uint32) for n in ("d", "heads", "kv_heads", "hd", "rot")] + [("theta", C.c_float)]
+                + [(n, C.c_uint32) for n in ("cols", "rows", "keys")] + [(n, C.c_void_p) for n in ("p", "p16", "o16", "k16", "v16")])
+
+
+class AttnW(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("out", C.c_void_p)]
+
+
+class AttnRows(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("seqs", C.c_uint32), ("a16", C.c_void_p), ("amax", C.c_void_p), ("sa", C.c_uint32), ("pos", C.c_void_p),
+                ("slot", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_uint32), ("out", C.c_void_p)]
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_layer_attention_prompt_chunks_and_steps(on, mc, pkg, e4m3):
+    """The C host side: a batch of prompts at once, the same in two chunks over the cache, and token by token: the three agree with
+    the 64-bit form of the whole and so with one another."""
+    pkg.build.build_host()
+    L = C.CDLL(pkg.build.HOST_LIB)
+    L.moe_attn_open.restype = C.c_bool
+    L.moe_attn_open.argtypes = [C.POINTER(Attn), C.c_void_p] + [C.c_uint32] * 5 + [C.c_float, C.c_uint32, C.c_uint32]
+    L.moe_attn_close.argtypes = [C.POINTER(Attn)]
+    L.moe_attn_prompt.argtypes = [C.POINTER(Attn), C.POINTER(mc.Kv), C.POINTER(AttnW), C.POINTER(AttnRows), C.c_void_p, C.c_void_p, C.c_uint32]
+    L.moe_attn_step.argtypes = [C.POINTER(Attn), C.POINTER(mc.Kv), C.POINTER(AttnW), C.POINTER(AttnRows), C.c_void_p, C.c_uint32]
+    d, h, g, hd, rot, theta, page = 256, 6, 2, 64, 32, 1e4, 16
+    gen, lengths = _gen(61), [40, 7, 65]
+    seqs, rows = len(lengths), sum(lengths)
+    cols = ((h + 2 * g) * hd + 127) // 128 * 128
+    x = _f16(gen, rows, d)
+    qkv, wo = torch.zeros(cols, d, device="cuda", dtype=torch.float16), _f16(gen, d, h * hd) * 0.05
+    qkv[:(h + 2 * g) * hd] = _f16(gen, (h + 2 * g) * hd, d) * 0.06
+    per = -(-max(lengths) // page)
+    kv = Cache(mc, gen, seqs * per, page, g, hd, e4m3)
+    table = torch.randperm(seqs * per, device="cuda", generator=gen).int().view(seqs, per)
+    place = torch.cat([torch.arange(n, device="cuda") for n in lengths])
+    seq = torch.cat([torch.full((n,), i, device="cuda") for i, n in enumerate(lengths)])
+    slot = (table[seq, place // page] * page + place % page).int()
+    q, w = Attn(), AttnW(qkv.data_ptr(), wo.data_ptr())
+    assert L.moe_attn_open(C.byref(q), on.p, d, h, g, hd, rot, theta, rows, rows) and q.cols == cols
+
+    # the 64-bit form; keys and values as the cache keeps them
+    p = (x.double() @ qkv.double().T)[:, :(h + 2 * g) * hd].view(rows, h + 2 * g, hd)
+    a = place.double()[:, None] * theta ** (-torch.arange(rot // 2, device="cuda", dtype=torch.float64) / (rot // 2))
+    lo, hi, c, s = p[:, :h + g, :rot // 2].clone(), p[:, :h + g, rot // 2:rot].clone(), a.cos()[:, None], a.sin()[:, None]
+    p[:, :h + g, :rot // 2], p[:, :h + g, rot // 2:rot] = lo * c - hi * s, hi * c + lo * s
+    step = 2.0 ** -4 if e4m3 else 2.0 ** -11   # half a step of what the cache keeps, relative
+
+    def rows_of(idx, out):
+        t = {"x": x[idx].contiguous(), "pos": place[idx].int().contiguous(), "slot": slot[idx].contiguous()}
+        r = AttnRows(len(idx), seqs, t["x"].data_ptr(), None, NO_SLOT, t["pos"].data_ptr(), t["slot"].data_ptr(), table.data_ptr(), per, out.data_ptr())
+        return r, t
+
+    def want(idx, cached):
+        out, tol = torch.empty(len(idx), d, device="cuda", dtype=torch.float64), torch.empty(len(idx), d, device="cuda", dtype=torch.float64)
+        for n, i in enumerate(idx.tolist()):
+            b = i - int(place[i])
+            o, mass, size = R.attention(p[i:i + 1, :h], p[b:i + 1, h:h + g], p[b:i + 1, h + g:], hd ** -0.5, i - b)
+            out[n] = o.view(-1) @ wo.double().T
+            # queries and keys off by half a step of fp16 (and the cache's) move a logit by that of sum |qk|, values theirs, the
+            # products' sums 2^-20 of their size; then the kernel's own error, the output's rounding and the second product's
+            rel = (step if cached else 2.0 ** -11) + 2.0 ** -11
+            e = R.bound(o, mass, size, hd, i - b + 1) + mass * (2 * rel * size[..., None] * 1.1 + rel) + 2.0 ** -18 * mass
+            tol[n] = e.view(-1) @ wo.double().abs().T * 1.01 + 1e-5
+        return out, tol
+
+    whole = torch.arange(rows, device="cuda")
+    out = torch.full((rows, d), 7.0, device="cuda")
+    r, keep = rows_of(whole, out)
+    cu = _starts(lengths)
+    L.moe_attn_prompt(C.byref(q), C.byref(kv.c), C.byref(w), C.byref(r), cu.data_ptr(), None, 0)
+    on.flush()
+    ref, tol = want(whole, False)
+    assert ((out.double() - ref).abs() <= tol).all()
+
+    # two chunks: the second one's keys come back out of the cache
+    first = [n // 3 for n in lengths]
+    for idx, lq, lk in ((whole[place < torch.tensor(first, device="cuda")[seq]], first, first),
+                        (whole[place >= torch.tensor(first, device="cuda")[seq]], [n - f for n, f in zip(lengths, first)], lengths)):
+        out = torch.full((len(idx), d), 7.0, device="cuda")
+        r, keep = rows_of(idx, out)
+        cu_q, cu_k = _starts(lq), _starts(lk)
+        L.moe_attn_prompt(C.byref(q), C.byref(kv.c), C.byref(w), C.byref(r), cu_q.data_ptr(), cu_k.data_ptr(), sum(lk))
+        on.flush()
+        ref, tol = want(idx, True)
+        assert ((out.double() - ref).abs() <= tol).all()
+
+    # a token at a time, the last seven of every sequence
+    for back in range(7, 0, -1):
+        idx = torch.tensor([sum(lengths[:i + 1]) - back for i in range(seqs)], device="cuda")
+        length = _u32([n - back + 1 for n in lengths])
+        out = torch.full((seqs, d), 7.0, device="cuda")
+        r, keep = rows_of(idx, out)
+        L.moe_attn_step(C.byref(q), C.byref(kv.c), C.byref(w), C.byref(r), length.data_ptr(), max(lengths))
+        on.flush()
+        ref, tol = want(idx, True)
+        assert ((out.double() - ref).abs() <= tol).all()
+    L.moe_attn_close(C.byref(q))
