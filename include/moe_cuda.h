@@ -76,7 +76,9 @@ typedef struct moe_cuda_ctx moe_cuda_ctx_t;
 /* mda_vkc_init (src/vkc.c:95-161): bind one device and one in-order queue.
  * stream = an existing cudaStream_t to enqueue on, or NULL to create one.
  * The context holds a work area of 512 KiB per SM (74 MiB) until it is
- * destroyed; without memory for it the calls that use it do with less.
+ * destroyed; without memory for it the calls that use it do with less, but for
+ * moe_cuda_attn_decode and moe_cuda_attn of several sequences, which then fail
+ * with MOE_ERR_NOMEM.
  * Returns NULL only if the context object itself cannot be made; otherwise
  * check moe_cuda_status(). */
 moe_cuda_ctx_t *moe_cuda_create(int device, void *stream);
@@ -222,8 +224,8 @@ void moe_cuda_dense(moe_cuda_ctx_t *c, const void *A16, const void *W, float *C,
  * [rows x stride], per row `heads` heads of hd columns (queries, keys, values in
  * turn).  In the first rot_heads heads the pairs (i, i + rot/2), i < rot/2, turn
  * by pos[row] * theta^(-2i/rot), the angle taken in 64 bits; all other columns
- * are only rounded.  out [rows x out_stride] fp16.  pos may be NULL if rot_heads
- * is 0.  hd % 8 == 0, rot % 8 == 0, rot <= hd, rot <= 512; stride % 4 == 0. */
+ * are only rounded.  out [rows x out_stride] fp16, apart from x.  pos may be NULL
+ * if rot_heads is 0.  hd % 8 == 0, rot % 8 == 0, rot <= hd, rot <= 512; stride % 4 == 0. */
 struct moe_pc_rope_t { uint32_t rows, heads, rot_heads, hd, rot, stride, out_stride; float theta; };
 void moe_cuda_rope(moe_cuda_ctx_t *c, const float *x, const uint32_t *pos, void *out, struct moe_pc_rope_t pc);
 

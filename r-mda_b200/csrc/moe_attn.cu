@@ -749,7 +749,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // The list of tile pairs, those with the most key blocks first (counting sort over 1024 classes of cost; the order within a
 // class does not matter to any result).
 constexpr uint32_t PLAN_THREADS = 1024, CLASSES = 1024;
-__global__ void __launch_bounds__(PLAN_THREADS) moe_attn_plan_kernel(AttnArgs a, uint32_t seqs, uint4 *plan, uint32_t *pairs) {
+__global__ void __launch_bounds__(PLAN_THREADS) moe_attn_plan_kernel(AttnArgs a, uint32_t seqs, uint4 *plan, uint32_t *pairs, uint32_t most_pairs) {
     __shared__ uint32_t place[CLASSES];
     __shared__ uint32_t warp_sum[32];
     __shared__ uint32_t most;
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_attn_plan_kernel(AttnArgs a,
                 p.left = lq - i;
                 const uint32_t n = min(CLASSES - 1u, blocks_of(p, a.tile_tokens).n / per), cls = CLASSES - 1u - n;
                 const uint32_t at = atomicAdd(&place[cls], 1u);
-                if (pass != 0) plan[at] = make_uint4(p.q_row, p.left, p.k_row, p.lk);
+                if (pass != 0 && at < most_pairs) plan[at] = make_uint4(p.q_row, p.left, p.k_row, p.lk);   // offsets that fall (denied above) may give more
             }
         }
         __syncthreads();
@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_attn_plan_kernel(AttnArgs a,
         uint32_t before = 0;
         for (uint32_t w = 0; w < warp; w += 1) before += warp_sum[w];
         place[threadIdx.x] = before + incl - mine;
-        if (threadIdx.x == PLAN_THREADS - 1u) *pairs = before + incl;
+        if (threadIdx.x == PLAN_THREADS - 1u) *pairs = min(before + incl, most_pairs);
         __syncthreads();
     }
 }
@@ -820,6 +820,7 @@ extern "C" void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k1
     const char *why = moe_attn_refusal(q16, k16, v16, cu_q, cu_k, o16, pc);
     MOE_REQUIRE(c, why == NULL, "%s", why);
     if (pc.rows_q == 0 || pc.seqs == 0) return;
+    moe_on_device on(c);
     AttnArgs a;
     a.cu_q = cu_q;
     a.cu_k = cu_k;
@@ -847,7 +848,6 @@ extern "C" void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k1
                !moe_tmap_heads_f16(c, &tv, v16, pc.rows_k, pc.kv_heads, pc.hd, pc.kv_stride, 1, BLOCK_KEYS, pc.hd / 64u)) {
         return;
     }
-    moe_on_device on(c);
     if (pc.seqs > 1u) {
         const size_t need = 256 + (size_t)pairs * sizeof(uint4);
         if (need > c->work_bytes) {
@@ -856,7 +856,7 @@ extern "C" void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k1
         }
         a.pairs = (const uint32_t *)c->work;
         a.plan = (const uint4 *)((uint8_t *)c->work + 256);
-        moe_run(c, moe_attn_plan_kernel, 1, PLAN_THREADS, 0, a, pc.seqs, (uint4 *)a.plan, (uint32_t *)a.pairs);
+        moe_run(c, moe_attn_plan_kernel, 1, PLAN_THREADS, 0, a, pc.seqs, (uint4 *)a.plan, (uint32_t *)a.pairs, (uint32_t)pairs);
         MOE_LAUNCHED(c);
     }
     const uint64_t items = pairs * pc.kv_heads;

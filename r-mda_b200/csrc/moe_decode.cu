@@ -712,6 +712,7 @@ extern "C" void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv,
     const char *why = moe_attn_decode_refusal(kv, q16, table, len, o16, pc);
     MOE_REQUIRE(c, why == NULL, "%s", why);
     if (pc.seqs == 0) return;
+    moe_on_device on(c);
     DecArgs a;
     a.k_scale = kv->k_scale;
     a.v_scale = kv->v_scale;
@@ -740,7 +741,6 @@ extern "C" void moe_cuda_attn_decode(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv,
     }
     a.split = (uint4 *)c->work;
     a.part = (float *)((uint8_t *)c->work + split_bytes);
-    moe_on_device on(c);
     const bool fp8 = kv->type == MOE_KV_E4M3, wide = a.group > 8u;
     if (kv->hd == 128u) {
         if (fp8) wide ? decode_launch<128, 2, true>(c, kv, a, 0) : decode_launch<128, 1, true>(c, kv, a, 1);

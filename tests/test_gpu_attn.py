@@ -487,6 +487,33 @@ def test_row_ranges_outside_the_tensors(mc, cu_q, cu_k):
     assert (out[8] == 7).all()
 
 
+def test_many_falling_offsets(mc):
+    """Offsets that go to and fro cover the rows many times over: more tiles than the list has room for."""
+    g = _gen(5)
+    q, k, out = _f16(g, 4096, 16 * 64), _f16(g, 16, 64), torch.empty(4096, 16 * 64, device="cuda", dtype=torch.float16)
+    a, b = _u32([0, 4096] * 200), _u32([0, 16] * 200)
+    _refused(mc, lambda c: c.attn(q.data_ptr(), k.data_ptr(), k.data_ptr(), a.data_ptr(), b.data_ptr(), out.data_ptr(), 399, 4096, 16, 16, 1, 64), "row range")
+
+
+def test_attn_without_keys(on):
+    _attn(on, _gen(6), [5], [0], 4, 2, 64)
+    _attn(on, _gen(6), [5, 300, 1], [0, 0, 0], 4, 2, 128)
+
+
+def test_work_on_another_current_device(mc):
+    """The calling thread's current device is left as it was, and the calls run on the context's."""
+    s = _calls_state(mc, 71, [40, 9])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    c = mc.Ctx(0, stream.cuda_stream)
+    with torch.cuda.device(torch.cuda.device_count() - 1):
+        _run_of_calls(c, s)
+        c.flush()
+        assert torch.cuda.current_device() == torch.cuda.device_count() - 1
+    assert not (s["od"] == 7).all()
+    c.close()
+
+
 def test_host_refusals_are_sticky(mc):
     with mc.Ctx(0) as c:
         c.check()
