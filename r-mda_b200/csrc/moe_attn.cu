@@ -8,7 +8,7 @@
 // its keys and values once, and a tile spans few tokens, which keeps what is computed above the diagonal small.  A CTA works
 // on two such tiles (256 rows) against the same key blocks of 128, so that one tile's softmax runs under the other's products.
 // Persistent CTAs, one per SM, walk a list of (tile pair, kv head), the longest first.  Roles:
-//   warp 0     loads Q (both tiles), K and V blocks by TMA, a block to a load
+//   warp 0     loads K and V blocks by TMA, a block to a load, and Q, each tile as soon as its last scores have been issued
 //   warps 1, 3 issue the tcgen05.mma of the first and the second tile: S into tensor memory, then per block P V into the output
 //              accumulator (P is read from tensor memory, where it overwrites its own S).  A warp of its own for each tile: a
 //              look at a barrier takes some 200 cycles, and one tile's looks hide under the other's products
@@ -25,6 +25,12 @@
 // end are looked through before their product: their non-finite values become 0 in shared memory, and if there were any,
 // the rows that do see them get them added at the end from global memory (a weight is positive, so infinities keep their sign).
 // A NaN score makes the row's maximum NaN, and with it the whole row.
+//
+// One B200: a prompt of 4096 (32 heads of 128, 4 kv heads) 123 us = 1120 TFLOP/s, 0.68 of the measured bf16 rate; one of 8192
+// 460 us = 1195 in short bursts and 540 = 1020 back to back, under the power cap; 13 prompts up to 1999 behind 517 cached
+// tokens (12 heads of 64) 104 us; 32 windows of 384 (16 heads of 128, 2 kv heads) 43.5 us.  On long prompts the tensor pipe is busy
+// 0.57 and the exp2 unit 0.43 of the time: what is left is the softmax's own turn, ~1700 cycles a tile and block.  Short
+// prompts are bound by the steps between items (~3500 cycles) and by blocks cut by the diagonal.
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 
@@ -53,7 +59,7 @@ template <uint32_t ST>
 struct __align__(8) AttnBars {
     uint64_t kv_full[ST], kv_empty[ST];
     uint64_t v_landed[ST];   // masked V blocks: loaded; warp 2 then arrives at kv_full
-    uint64_t q_full, q_empty;
+    uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];   // p_full: of each tile, keys 0-63 and 64-127
     uint64_t sum_full[2], sum_empty[2];
     uint64_t turn[2];        // the tile's softmax may begin: the other one's has ended
@@ -283,8 +289,10 @@ __device__ __forceinline__ void store32(__half *to, const uint32_t (&w)[8], bool
     }
 }
 
-// mbar_wait without a call, so that the registers of a softmax thread need not follow a calling convention.
-__device__ __forceinline__ bool wait_here(uint32_t bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t site, uint64_t wait_ns) {
+// mbar_wait in two parts: the first looks stand where the wait is (a call would hold a softmax thread's registers to a calling
+// convention), all that bounds it is out of line.  Each role's step from item to item runs code that the others' have pushed
+// out of the instruction cache, so the code is kept short: 32 windows of 384 take 43.5 us, with the whole wait in every place 47.3.
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t site, uint64_t wait_ns) {
     uint32_t spins = 0;
     uint64_t t0 = 0;
     while (!mbar_try_wait(bar, parity)) {
@@ -301,6 +309,14 @@ __device__ __forceinline__ bool wait_here(uint32_t bar, uint32_t parity, volatil
         }
     }
     return true;
+}
+
+__device__ __forceinline__ bool wait_here(uint32_t bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t site, uint64_t wait_ns) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < 64u; i += 1) {
+        if (mbar_try_wait(bar, parity)) return true;
+    }
+    return wait_long(bar, parity, abort, status, site, wait_ns);
 }
 
 template <uint32_t HD>
@@ -322,9 +338,9 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             mbar_init(smem_u32(&bars->kv_empty[i]), 2);
             mbar_init(smem_u32(&bars->v_landed[i]), 1);
         }
-        mbar_init(smem_u32(&bars->q_full), 1);
-        mbar_init(smem_u32(&bars->q_empty), 2);
         for (uint32_t i = 0; i < 2; i += 1) {
+            mbar_init(smem_u32(&bars->q_full[i]), 1);
+            mbar_init(smem_u32(&bars->q_empty[i]), 1);
             mbar_init(smem_u32(&bars->s_full[i]), 1);
             mbar_init(smem_u32(&bars->p_full[i][0]), TILE_ROWS);
             mbar_init(smem_u32(&bars->p_full[i][1]), TILE_ROWS);
@@ -364,7 +380,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (warp == 0) {
             // ---------------- loads: ring places K(n-1), V(n-1), K(n-2), V(n-2), ... of each item in turn ----------------
             if (lane == 0) {
-                uint32_t at = 0, q_phase = 1, issued = 0, parity = 0, masked = 0, landed = 0, q_loads = 0;
+                uint32_t at = 0, issued = 0, parity = 0, masked = 0, landed = 0, q_loads[2] = {0, 0};
                 bool ok = true;
                 while (ok && items.next(a, p, head)) {
                     const Blocks b = blocks_of(p, a.tile_tokens);
@@ -372,21 +388,6 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     for (uint32_t i = 0; i < 2u * b.n; i += 1) {
                         const uint32_t j = b.n - 1u - i / 2u, s = at % ST, ph = (at / ST) & 1u;
                         const bool is_v = (i & 1u) != 0;
-                        if (i == 0) {
-                            if (!AT_WAIT(&bars->q_empty, q_phase, 31)) {
-                                ok = false;
-                                break;
-                            }
-                            q_phase ^= 1u;
-                            mbar_expect_tx(smem_u32(&bars->q_full), a.group * a.tile_tokens * HD * 2u * (b.has_b ? 2u : 1u));
-                            // a group of an odd size leaves rows of the tile free, so each half is placed by itself
-                            for (uint32_t x = 0; x < (b.has_b ? 2u : 1u) * C::HALVES; x += 1) {
-                                const uint32_t tile = x / C::HALVES, half = x % C::HALVES;
-                                tma_load_4d(q_smem + tile * C::TILE_BYTES + half * HALF_BYTES, &tm_q, smem_u32(&bars->q_full),
-                                            (int32_t)(head * a.group), (int32_t)(p.q_row + tile * a.tile_tokens), (int32_t)half);
-                            }
-                            q_loads += 1;
-                        }
                         if (!AT_WAIT(&bars->kv_empty[s], ph ^ 1u, 32)) {
                             ok = false;
                             break;
@@ -400,6 +401,21 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                         masked = (masked & ~(1u << s)) | ((m ? 1u : 0u) << s);
                         landed ^= (m ? 1u : 0u) << s;   // the next masked use's parity
                         at += 1u;
+                        // Q behind the item's first two blocks, for which there is room earlier
+                        for (uint32_t tile = 0; tile < 2u && i == 1 && ok; tile += 1) {
+                            if (b.tile[tile] == 0) continue;
+                            const uint32_t q_bar = smem_u32(&bars->q_full[tile]);
+                            ok = AT_WAIT(&bars->q_empty[tile], ~q_loads[tile] & 1u, 31);
+                            if (!ok) break;
+                            mbar_expect_tx(q_bar, a.group * a.tile_tokens * HD * 2u);
+                            // a group of an odd size leaves rows of the tile free, so each half is placed by itself
+                            for (uint32_t half = 0; half < C::HALVES; half += 1) {
+                                tma_load_4d(q_smem + tile * C::TILE_BYTES + half * HALF_BYTES, &tm_q, q_bar, (int32_t)(head * a.group),
+                                            (int32_t)(p.q_row + tile * a.tile_tokens), (int32_t)half);
+                            }
+                            q_loads[tile] += 1;
+                        }
+                        if (!ok) break;
                     }
                 }
                 if (*abort != 0) {
@@ -413,8 +429,10 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                             }
                         }
                     }
-                    for (uint32_t spin = 0; q_loads != 0 && spin < (1u << 16); spin += 1) {
-                        if (mbar_try_wait(smem_u32(&bars->q_full), (q_loads - 1u) & 1u)) break;
+                    for (uint32_t tile = 0; tile < 2; tile += 1) {
+                        for (uint32_t spin = 0; q_loads[tile] != 0 && spin < (1u << 16); spin += 1) {
+                            if (mbar_try_wait(smem_u32(&bars->q_full[tile]), (q_loads[tile] - 1u) & 1u)) break;
+                        }
                     }
                 }
             }
@@ -441,7 +459,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                         umma_commit(smem_u32(&bars->s_full[t]));
                     }
                     umma_commit(smem_u32(&bars->kv_empty[slot]));
-                    if (last) umma_commit(smem_u32(&bars->q_empty));
+                    if (last && mine) umma_commit(smem_u32(&bars->q_empty[t]));
                 }
                 __syncwarp();
             };
@@ -449,10 +467,10 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 const Blocks b = blocks_of(p, a.tile_tokens);
                 if (b.n == 0) continue;
                 uint32_t ks = at % ST;
-                ok = AT_WAIT(&bars->q_full, q_phase, 33) && AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34);
+                ok = AT_WAIT(&bars->kv_full[ks], (at / ST) & 1u, 34) && (b.tile[t] == 0 || AT_WAIT(&bars->q_full[t], q_phase, 33));
                 __syncwarp();
                 if (!ok) break;
-                q_phase ^= 1u;
+                if (b.tile[t] != 0) q_phase ^= 1u;
                 scores(ks, b.n == b.tile[t], b.n == 1u);
                 for (uint32_t j = b.n; j-- > 0;) {
                     const uint32_t vi = at + 1u, vs = vi % ST;
@@ -518,12 +536,16 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     landed ^= 1u << vs;
                     __syncwarp();
                     uint8_t *block = smem + (2u + vs) * C::TILE_BYTES;
-                    uint32_t most = 0;   // the largest exponent and mantissa of either half
-#pragma unroll 4
+                    uint32_t top[4] = {0, 0, 0, 0};   // the largest exponents and mantissas of both halves
+#pragma unroll 8
                     for (uint32_t i = lane; i < C::TILE_BYTES / 16u; i += 32u) {
                         const uint4 w = *reinterpret_cast<const uint4 *>(block + i * 16u);
-                        most = __vmaxu2(__vmaxu2(__vmaxu2(most, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, w.z & 0x7fff7fffu)), w.w & 0x7fff7fffu);
+                        top[0] = __vmaxu2(top[0], w.x & 0x7fff7fffu);
+                        top[1] = __vmaxu2(top[1], w.y & 0x7fff7fffu);
+                        top[2] = __vmaxu2(top[2], w.z & 0x7fff7fffu);
+                        top[3] = __vmaxu2(top[3], w.w & 0x7fff7fffu);
                     }
+                    const uint32_t most = __vmaxu2(__vmaxu2(top[0], top[1]), __vmaxu2(top[2], top[3]));
                     if (__any_sync(0xffffffffu, (most & 0xffffu) >= 0x7c00u || (most >> 16) >= 0x7c00u)) {
                         for (uint32_t i = lane; i < C::TILE_BYTES / 4u; i += 32u) {
                             uint32_t *w = reinterpret_cast<uint32_t *>(block + i * 4u);
@@ -566,21 +588,12 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     break;
                 }
                 s_phase ^= 1u;
-                // The two tiles' softmaxes take turns, block by block: alone on the SM's units one is done twice as fast, and
-                // the other one's products run meanwhile.  Left to themselves they fall into step.
-                const bool turns = j < both;
-                if (turns) {
-                    if (!AT_WAIT(&bars->turn[t], turn_phase, 45)) {
-                        ok = false;
-                        break;
-                    }
-                    turn_phase ^= 1u;
-                }
                 __syncwarp();
                 tc_fence_after();
                 if ((int32_t)((j + 1u) * BLOCK_KEYS) > tile_first) {
                     // some rows do not see all of the block: what they do not see becomes -infinity where it lies, so that the code
-                    // below, which every block runs, is short (straight through once a block, it is bound by its own fetching)
+                    // below, which every block runs, is short (straight through once a block, it is bound by its own fetching); done
+                    // while the other tile has its turn
                     const int32_t seen = vis - (int32_t)(j * BLOCK_KEYS);   // columns below it are visible
 #pragma unroll 1
                     for (int32_t i = 0; i < 4; i += 1) {
@@ -596,6 +609,17 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     }
                     tmem_st_wait();
                 }
+                // The two tiles' softmaxes take turns, block by block (masks come before): alone on the SM's units one is done twice as fast, and
+                // the other one's products run meanwhile.  Left to themselves they fall into step.
+                const bool turns = j < both;
+                if (turns) {
+                    if (!AT_WAIT(&bars->turn[t], turn_phase, 45)) {
+                        ok = false;
+                        break;
+                    }
+                    turn_phase ^= 1u;
+                }
+                __syncwarp();
                 // Scores are read twice, 32 columns at a time and each piece while the one before it is worked on: a whole row in
                 // registers would cost the other warps theirs.
                 uint32_t s[2][32];

@@ -12,7 +12,12 @@
 // Scores are computed as S^T = K Q^T (16 tokens x 8 heads x 16 columns per mma.sync) and outputs as O^T = V^T P^T, so groups
 // of up to 8 heads waste nothing; P^T comes from S^T's accumulators by an 8x8 transpose (movmatrix).  Operands come from shared
 // memory by ldmatrix: fp16 as they are; of e4m3 a lane gets two pairs of neighbouring columns, which are converted in
-// registers (the order of K's columns inside a product is free, Q's is the same).
+// registers (the order of K's columns inside a product is free, Q's is the same).  A group is 8 of the 64 rows that the
+// 5th-generation tensor cores' smallest product has, and the products are far from a bound here.
+//
+// One B200: 129 sequences of up to 8191 tokens, fp16, 4 kv heads of 128 (1.08 GB) 171 us, of which this kernel 166 = 6.5 TB/s, the
+// copy rate; 16 of up to 16384, e4m3 (141 MB) 36.7 us, bound by instructions (codes to fp16) and ~7 us of join and gaps; one of
+// 777 tokens 9.5 us with the call, a chain of latencies: the line, the first loads, the joins.
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 
