@@ -27,8 +27,8 @@
 // A NaN score makes the row's maximum NaN, and with it the whole row.
 //
 // One B200: a prompt of 4096 (32 heads of 128, 4 kv heads) 123 us = 1120 TFLOP/s, 0.68 of the measured bf16 rate; one of 8192
-// 460 us = 1195 in short bursts and 540 = 1020 back to back, under the power cap; 13 prompts up to 1999 behind 517 cached
-// tokens (12 heads of 64) 104 us; 32 windows of 384 (16 heads of 128, 2 kv heads) 43.5 us.  On long prompts the tensor pipe is busy
+// 460 us = 1195 in short bursts and 533 = 1030 back to back, under the power cap; 13 prompts up to 1999 behind 517 cached
+// tokens (12 heads of 64) 104 us; 32 windows of 384 (16 heads of 128, 2 kv heads) 43.5 us (both captured, with the plan kernel).  On long prompts the tensor pipe is busy
 // 0.57 and the exp2 unit 0.43 of the time: what is left is the softmax's own turn, ~1700 cycles a tile and block.  Short
 // prompts are bound by the steps between items (~3500 cycles) and by blocks cut by the diagonal.
 #include "moe_attn.cuh"
