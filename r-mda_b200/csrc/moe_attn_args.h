@@ -9,6 +9,16 @@
 
 #define MOE_ATTN_MAX_GROUP 16u
 
+#ifdef __CUDACC__
+#define MOE_BOTH __host__ __device__
+#else
+#define MOE_BOTH
+#endif
+
+/* Parts that decode's join reads of a head which begins in SM `first`'s piece, of `sms` parts there are: n, or none if they
+ * would pass the last.  What a piece that gave up leaves behind may be any number. */
+MOE_BOTH static inline uint32_t moe_join_parts(uint32_t first, uint32_t n, uint32_t sms) { return first < sms && n <= sms - first ? n : 0u; }
+
 static inline int moe_at16(const void *p) { return p != NULL && ((uintptr_t)p & 15u) == 0; }
 static inline int moe_at4(const void *p) { return p != NULL && ((uintptr_t)p & 3u) == 0; }
 

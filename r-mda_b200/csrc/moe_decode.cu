@@ -174,10 +174,16 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     __shared__ uint2 ended_of[DEC_WARPS], goes_on_of[DEC_WARPS];   // sequence and kv head; a sequence of ~0: none
     __shared__ bool begins[DEC_WARPS];   // the last one begins in the warp's piece
     __shared__ uint32_t behind;          // stages of the SM's last head behind its piece
+    __shared__ bool gave_up;             // some warp's wait ran out: what it leaves is incomplete, `behind` may not have been written
     __shared__ uint4 over;               // the head that begins in the SM's piece and goes on behind it: sequence, kv head, first SM, SMs
     if (lane < St::COUNT) {
         mbar_init(bars0 + lane * 8u, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 0) {
+        over = make_uint4(0, 0, 0, 0);
+        behind = 0;
+        gave_up = false;
     }
     moe_pdl_begin();
 
@@ -243,7 +249,6 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         p.len = a.len[p.s];
     }
 
-    if (threadIdx.x == 0) over = make_uint4(0, 0, 0, 0);
     auto sm_of = [&](unsigned long long x) { return piece_of(x, total, sms); };
     Place q = p;             // the next stage to load, and the pages of its boxes
     uint32_t to_load = left, pg[SG];
@@ -562,6 +567,7 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     }
     if (FP8) asm volatile("cp.async.wait_all;" ::: "memory");
     if (left != 0) {   // gave up: a bounded time for the copies in flight
+        gave_up = true;
         for (uint32_t spin = 0; spin < (1u << 16); spin += 1) {
             bool done = true;
             for (uint32_t i = 0; i < St::COUNT; i += 1) done = mbar_try_wait(bars0 + i * 8u, i >= place ? phase : phase ^ 1u) && done;
@@ -624,7 +630,7 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                 }
             }
         }
-        if (here && !ends && threadIdx.x == 0) over = make_uint4(key.x, key.y, blockIdx.x, sm_of(sm1 + behind - 1u) - blockIdx.x + 1u);
+        if (here && !ends && !gave_up && threadIdx.x == 0) over = make_uint4(key.x, key.y, blockIdx.x, sm_of(sm1 + behind - 1u) - blockIdx.x + 1u);
     }
     if (ended_of[0].x != ~0u) {   // begun in an earlier SM's piece, ended in this one's first warp
         for (uint32_t i = threadIdx.x; i < a.group * (HD + 2u); i += DEC_THREADS) begun_earlier[i] = ended[i];
@@ -648,8 +654,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) moe_attn_join_kernel(DecArgs 
     moe_pdl_begin();
     const uint32_t first = blockIdx.x / a.group, head = blockIdx.x - first * a.group;
     const uint4 split = a.split[first];   // sequence, kv head, first SM, SMs
-    if (split.w == 0u) return;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, size = part_floats(a.group, HD), n = split.w;
+    const uint32_t n = moe_join_parts(first, split.w, gridDim.x / a.group);
+    if (n == 0u) return;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, size = part_floats(a.group, HD);
     auto part_at = [&](uint32_t i) { return a.part + (size_t)((first + i) * 2u + (i == 0 ? 1u : 0u)) * size; };
     const uint32_t at_top = a.group * HD + head, at_sum = a.group * (HD + 1u) + head;
     float m = -INFINITY, sum = 0.0f;
