@@ -45,7 +45,9 @@ constexpr float GROW = 6.0f;                     // log2 of how far weights may 
 constexpr float SHIFT = 8.0f;                    // weights are at most 2^(GROW + SHIFT) = 2^14; fp16 then goes down to 2^-32 of the reference
 // Of every POLY_OF pairs of exponentials POLY_SHARE go to the multiply-add pipe.
 constexpr uint32_t POLY_OF = 4, POLY_SHARE = 1;
-constexpr uint32_t FLAGS = 8;                    // items that may be between their V check and their epilogue
+// Items with a masked block that may be between their V check and their epilogue.  Each has such a block in the ring until its products
+// are done: four items in a ring of eight places, one more per tile whose output has not been stored, and the one whose check begins.
+constexpr uint32_t FLAGS = 8;
 
 template <uint32_t HD>
 struct Cfg {
@@ -153,6 +155,7 @@ struct Blocks {
     bool has_b;
     uint32_t n;
     int32_t masked_from;  // blocks from here on are masked for some row
+    __device__ __forceinline__ bool masks() const { return masked_from < (int32_t)n; }
 };
 __device__ __forceinline__ Blocks blocks_of(const Pair &p, uint32_t tile_tokens) {
     Blocks b;
@@ -523,7 +526,10 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             bool ok = true;
             while (ok && items.next(a, p, head)) {
                 const Blocks b = blocks_of(p, a.tile_tokens);
-                if (b.n == 0) continue;
+                if (!b.masks()) {   // no wait here holds this warp back: an item without a masked block has no flag
+                    at += 2u * b.n;
+                    continue;
+                }
                 volatile uint32_t *found = &bars->found[n_item % FLAGS];
                 if (lane == 0) *found = 0;
                 __syncwarp();
@@ -709,7 +715,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         while (ok && items.next(a, p, head)) {
             const Blocks b = blocks_of(p, a.tile_tokens);
             const uint32_t flag = n_item % FLAGS;
-            if (b.n != 0) n_item += 1;
+            if (b.masks()) n_item += 1;
 #pragma unroll
             for (uint32_t t = 0; t < 2; t += 1) {
                 const uint32_t token = t * a.tile_tokens + my_token;   // behind the pair's first
@@ -730,7 +736,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 const float sum = bars->sum[t][row];
                 mbar_arrive(smem_u32(&bars->sum_empty[t]));
                 const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const bool extra = *(volatile uint32_t *)&bars->found[flag] != 0;
+                const bool extra = b.masks() && *(volatile uint32_t *)&bars->found[flag] != 0;
                 const int32_t vis = visible(p, token);
 #pragma unroll 1
                 for (uint32_t i = 0; i < HD / 16u; i += 1) {
