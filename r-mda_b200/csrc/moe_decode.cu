@@ -191,7 +191,14 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     const uint32_t share = (a.seqs + DEC_THREADS - 1u) / DEC_THREADS;
     const uint32_t s_lo = min(threadIdx.x * share, a.seqs), s_hi = min(s_lo + share, a.seqs);
     unsigned long long mine = 0;
-    for (uint32_t s = s_lo; s < s_hi; s += 1) mine += stages_of(a, s, PER);
+    for (uint32_t s = s_lo; s < s_hi; s += 1) {
+        const uint32_t n = a.len[s];
+        if (n > a.max_len) {
+            if (blockIdx.x == 0) moe_deny(a.status, MOE_SITE_LENGTH);   // here, before any return
+        } else {
+            mine += (n + PER - 1u) / PER;
+        }
+    }
     unsigned long long incl = mine;
 #pragma unroll
     for (uint32_t o = 1; o < 32; o <<= 1) {
@@ -636,11 +643,6 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         for (uint32_t i = threadIdx.x; i < a.group * (HD + 2u); i += DEC_THREADS) begun_earlier[i] = ended[i];
     }
 
-    if (blockIdx.x == 0) {
-        for (uint32_t s = s_lo; s < s_hi; s += 1) {
-            if (a.len[s] > a.max_len) moe_deny(a.status, MOE_SITE_LENGTH);
-        }
-    }
     if (threadIdx.x == 0) a.split[blockIdx.x] = over;
 }
 

@@ -37,3 +37,15 @@ def test_attn_infinity_before_many_unmasked_items(on, hd, value):
             o[:, :, 5] = 0
         R.check(out[i:i + 1], o, mass, size, hd, n)
         at += n
+
+
+# ---- refusals that only the device can see --------------------------------------------------------
+@pytest.mark.parametrize("lengths", [[33], [0xFFFFFFFF], [0xFFFFFFFF, 0], [0, 33, 0, 0x80000000]])
+def test_lengths_beyond_the_bound_with_nothing_else_to_do(mc, lengths):
+    """Every sequence refused or empty: zeros, and the status says so."""
+    seqs = len(lengths)
+    kv = Cache(mc, _gen(3), 4, 16, 1, 64, False)
+    table, length = torch.zeros(seqs, 2, device="cuda", dtype=torch.int32), _u32(lengths)
+    q, out = _f16(_gen(4), seqs, 64), torch.full((seqs + 1, 64), 7.0, device="cuda", dtype=torch.float16)
+    _refused(mc, lambda c: c.attn_decode(kv.c, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), seqs, 1, 32, 2), "length")
+    assert (out[:seqs] == 0).all() and (out[seqs:] == 7).all()
