@@ -216,8 +216,8 @@ void moe_cuda_dense(moe_cuda_ctx_t *c, const void *A16, const void *W, float *C,
  * be captured into a graph; the attentions use the context's work area, so
  * graphs captured from one context must not run at the same time.
  * Sizes that the host knows are refused with MOE_ERR_ARG before anything runs.
- * What only the device can see (a slot, page or length out of its range) is
- * skipped without an access, and the status becomes MOE_ERR_ARG by the next
+ * What only the device can see (a slot, page, length or row offset out of its
+ * range) is skipped without an access, and the status becomes MOE_ERR_ARG by the next
  * flush. */
 
 /* Rotary positions, and the fp32 -> fp16 rounding of all three operands: x fp32
@@ -255,7 +255,8 @@ void moe_cuda_kv_write(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const void *k
 /* Back out of the cache, as moe_cuda_attn takes them: rows cu[s] .. cu[s+1]-1 of
  * k16 and v16 ([rows x stride]) become places 0, 1, ... of sequence s, whose
  * pages are table[s * table_stride + place / page].  cu[seqs + 1] never falls;
- * rows from cu[seqs] on, and rows whose page is refused, are left as they were. */
+ * rows before cu[0], from cu[seqs] on, and rows whose page is refused or whose
+ * sequence passes `rows`, are left as they were. */
 struct moe_pc_kv_read_t { uint32_t seqs, rows, table_stride, stride; };
 void moe_cuda_kv_read(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const uint32_t *table, const uint32_t *cu, void *k16, void *v16,
                       struct moe_pc_kv_read_t pc);

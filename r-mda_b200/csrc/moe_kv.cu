@@ -219,25 +219,38 @@ __global__ void __launch_bounds__(KV_THREADS, 6) moe_kv_read_kernel(const uint32
                                                                   moe_pc_kv_read_t pc, uint32_t tile) {
     __shared__ uint32_t slots[2][READ_ROWS];
     moe_pdl_begin();
-    const uint32_t last = min(cu[pc.seqs], pc.rows);
+    const uint32_t total_rows = cu[pc.seqs], last = min(total_rows, pc.rows);
     const uint32_t lane = threadIdx.x % LPV;
+    // Offsets that fall or pass the rows are refused: a thread loads those of a sequence here and looks at them at the end.
+    uint32_t mine = blockIdx.x * KV_THREADS + threadIdx.x, begin = 0, end = 0;
+    if (mine < pc.seqs) {
+        begin = cu[mine];
+        end = cu[mine + 1u];
+    }
     // Slots of a tile's rows, a row per thread; those of the next tile are looked up while this one is copied.
     auto look_up = [&](uint64_t r0, uint32_t *to) {
         if (threadIdx.x >= tile || r0 + threadIdx.x >= last) return;
         const uint32_t r = (uint32_t)r0 + threadIdx.x;
-        uint32_t lo = 0, hi = pc.seqs;  // the sequence of row r: cu[lo] <= r < cu[hi]
+        uint32_t lo = 0, hi = pc.seqs, stop = total_rows;  // the sequence of row r: cu[lo] <= r < cu[hi] = stop
         while (hi - lo > 1u) {
-            const uint32_t mid = (lo + hi) / 2u;
-            if (cu[mid] <= r) lo = mid;
-            else hi = mid;
+            const uint32_t mid = (lo + hi) / 2u, at = cu[mid];
+            if (at <= r) {
+                lo = mid;
+            } else {
+                hi = mid;
+                stop = at;
+            }
         }
         const uint32_t first = cu[lo], place = r - first;
         uint32_t s = MDA_PC_NO_SLOT;
-        if (r >= first && place >> kv.page_shift < pc.table_stride) {
-            const uint32_t pg = table[(size_t)lo * pc.table_stride + (place >> kv.page_shift)];
-            if (pg < kv.pages) s = (pg << kv.page_shift) + (place & (kv.page - 1u));
+        // rows before the first sequence are no one's, and a sequence that passes the rows (refused at the end) is left
+        if (r >= first && stop <= pc.rows) {
+            if (place >> kv.page_shift < pc.table_stride) {
+                const uint32_t pg = table[(size_t)lo * pc.table_stride + (place >> kv.page_shift)];
+                if (pg < kv.pages) s = (pg << kv.page_shift) + (place & (kv.page - 1u));
+            }
+            if (s == MDA_PC_NO_SLOT) moe_deny(kv.status, MOE_SITE_PAGE);
         }
-        if (s == MDA_PC_NO_SLOT) moe_deny(kv.status, MOE_SITE_PAGE);
         to[threadIdx.x] = s;
     };
     uint32_t buf = 0;
@@ -282,6 +295,13 @@ __global__ void __launch_bounds__(KV_THREADS, 6) moe_kv_read_kernel(const uint32
                 *reinterpret_cast<uint4 *>(v16 + to[j]) = FP8 ? from_e4m3(make_uint2(y[j].x, y[j].y), vs[j]) : y[j];
             }
         }
+    }
+    while (mine < pc.seqs) {
+        if (begin > end || end > pc.rows) moe_deny(kv.status, MOE_SITE_ROWS);
+        mine += gridDim.x * KV_THREADS;
+        if (mine >= pc.seqs) break;
+        begin = cu[mine];
+        end = cu[mine + 1u];
     }
 }
 

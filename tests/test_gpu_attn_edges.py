@@ -49,3 +49,34 @@ def test_lengths_beyond_the_bound_with_nothing_else_to_do(mc, lengths):
     q, out = _f16(_gen(4), seqs, 64), torch.full((seqs + 1, 64), 7.0, device="cuda", dtype=torch.float16)
     _refused(mc, lambda c: c.attn_decode(kv.c, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), seqs, 1, 32, 2), "length")
     assert (out[:seqs] == 0).all() and (out[seqs:] == 7).all()
+
+
+@pytest.mark.parametrize("cu,rows,read,left", [([0, 20, 50], 40, (0, 20), (20, 40)), ([0, 41], 40, None, (0, 40)), ([0, 30, 10, 40], 40, None, None),
+                                               ([50, 60], 40, None, (0, 40)), ([0xFFFFFFF0, 5], 40, None, (0, 40))])
+def test_kv_read_ranges_outside_the_rows(mc, cu, rows, read, left):
+    """Offsets that fall or pass the rows: the status says so, rows of such a sequence are left, nothing behind the rows is written."""
+    kv = Cache(mc, _gen(5), 5, 16, 2, 64, False)
+    table = torch.arange(5, device="cuda", dtype=torch.int32).repeat(len(cu) - 1, 1).contiguous()
+    k, v = (torch.full((rows + 3, 128), 7.0, device="cuda", dtype=torch.float16) for _ in range(2))
+    at = _u32(cu)
+    _refused(mc, lambda c: c.kv_read(kv.c, table.data_ptr(), at.data_ptr(), k.data_ptr(), v.data_ptr(), len(cu) - 1, rows, 5), "row range")
+    assert (k[rows:] == 7).all() and (v[rows:] == 7).all()
+    if left is not None:
+        assert (k[left[0]:left[1]] == 7).all() and (v[left[0]:left[1]] == 7).all()
+    if read is not None:
+        want = kv.rows(torch.arange(5, device="cuda"), read[1])
+        for t, w in zip((k, v), want):
+            assert torch.equal(t[read[0]:read[1]].view(-1, 2, 64), w.half())
+
+
+def test_kv_read_rows_before_the_first_sequence(on, mc):
+    """Offsets that begin behind 0, as moe_cuda_attn takes them: the rows before are left, and nothing is wrong."""
+    kv = Cache(mc, _gen(6), 3, 16, 2, 64, True)
+    table = torch.tensor([[2, 0, 1]], device="cuda", dtype=torch.int32)
+    k, v = (torch.full((50, 128), 7.0, device="cuda", dtype=torch.float16) for _ in range(2))
+    cu = _u32([9, 49])
+    on.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), 1, 50, 3)
+    on.flush()
+    for t, w in zip((k, v), kv.rows(table[0].long(), 40)):
+        assert torch.equal(t[9:49].view(40, 2, 64), w.half())
+        assert (t[:9] == 7).all() and (t[49:] == 7).all()
