@@ -244,10 +244,12 @@ typedef struct moe_cuda_kv_t {
 
 /* rows of k16 and v16 ([rows x stride], kv_heads * hd columns used) into the
  * slots slot[row] (MDA_PC_NO_SLOT: this row is not kept).  e4m3: the scale is the
- * least power of two with amax <= 448 * scale (1 for zeros), so that reading back
- * to fp16 is exact for normal fp16 values; rounding to nearest even; a NaN stays
- * NaN and does not enter amax; infinities count as 65504 there and read back as
- * infinities.  Two rows with one slot: either may be kept, head by head. */
+ * least power of two with amax <= 448 * scale (1 for zeros), so that scaling
+ * rounds nothing; values round once, to e4m3's nearest even.  63488 to 65504 are
+ * kept as 65536 and read back as 65504.  A NaN stays NaN and does not enter amax.
+ * Infinities count as 65504 there, are kept as 448 * 256 and read back as
+ * infinities; moe_cuda_attn_decode takes code * scale as it is, so there they
+ * count as 114688 and the largest fp16 values as 65536.  Two rows with one slot: either may be kept, head by head. */
 struct moe_pc_kv_write_t { uint32_t rows, stride; };
 void moe_cuda_kv_write(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const void *k16, const void *v16, const uint32_t *slot,
                        struct moe_pc_kv_write_t pc);
@@ -256,7 +258,8 @@ void moe_cuda_kv_write(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const void *k
  * k16 and v16 ([rows x stride]) become places 0, 1, ... of sequence s, whose
  * pages are table[s * table_stride + place / page].  cu[seqs + 1] never falls;
  * rows before cu[0], from cu[seqs] on, and rows whose page is refused or whose
- * sequence passes `rows`, are left as they were. */
+ * sequence passes `rows`, are left as they were.  e4m3: code * scale, rounded once;
+ * what lies between 65504 and 65536 is 65504, what lies beyond is infinite. */
 struct moe_pc_kv_read_t { uint32_t seqs, rows, table_stride, stride; };
 void moe_cuda_kv_read(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const uint32_t *table, const uint32_t *cu, void *k16, void *v16,
                       struct moe_pc_kv_read_t pc);

@@ -192,13 +192,17 @@ __global__ void __launch_bounds__(KV_THREADS, 8) moe_kv_write_kernel(const __hal
     }
 }
 
+// code * scale in fp16's range.  fp16 values of an amax above 57344 are kept at scale 256, and 63488 to 65504 of them round to code
+// 256: 65536, which is no fp16 value, reads as the largest one.  What lies beyond is infinite: an infinity is kept as 448 * 256.
+__device__ __forceinline__ float in_f16(float y) { return fabsf(y) <= 65536.0f ? fminf(fmaxf(y, -65504.0f), 65504.0f) : y; }
+
 // Eight codes as fp16 values of code * scale, rounded once.
 __device__ __forceinline__ uint4 from_e4m3(uint2 c, float scale) {
     uint32_t o[4];
     e4m3x4_to_h2(c.x, o[0], o[1]);
     e4m3x4_to_h2(c.y, o[2], o[3]);
     const uint32_t bits = __float_as_uint(scale), e = bits >> 23;
-    if ((bits & 0x807fffffu) == 0u && e >= 127u - 14u && e <= 127u + 15u) {   // a power of two that fp16 has: one rounding all the same
+    if ((bits & 0x807fffffu) == 0u && e >= 127u - 14u && e <= 127u + 7u) {   // a power of two that fp16 has, 448 of it too: one rounding all the same
         const __half2 f = __half2half2(__ushort_as_half((unsigned short)((e - 112u) << 10)));
 #pragma unroll
         for (uint32_t i = 0; i < 4; i += 1) o[i] = as_word(__hmul2(as_h2(o[i]), f));
@@ -206,7 +210,7 @@ __device__ __forceinline__ uint4 from_e4m3(uint2 c, float scale) {
 #pragma unroll
         for (uint32_t i = 0; i < 4; i += 1) {
             const float2 y = __half22float2(as_h2(o[i]));
-            o[i] = as_word(__floats2half2_rn(y.x * scale, y.y * scale));
+            o[i] = as_word(__floats2half2_rn(in_f16(y.x * scale), in_f16(y.y * scale)));
         }
     }
     return make_uint4(o[0], o[1], o[2], o[3]);

@@ -80,3 +80,52 @@ def test_kv_read_rows_before_the_first_sequence(on, mc):
     for t, w in zip((k, v), kv.rows(table[0].long(), 40)):
         assert torch.equal(t[9:49].view(40, 2, 64), w.half())
         assert (t[:9] == 7).all() and (t[49:] == 7).all()
+
+
+# ---- the ends of the types ---------------------------------------------------------------------------
+@pytest.mark.parametrize("hd", [64, 128])
+def test_largest_values_through_an_e4m3_cache(on, mc, hd):
+    """fp16 values up to 65504 come back finite: those that are kept as 256 * 256 as 65504.  Infinities come back as infinities."""
+    x = torch.zeros(6, hd, device="cuda", dtype=torch.float16)
+    x[0, :8] = torch.tensor([65504.0, -65504.0, 63488.0, 63456.0, 61440.0, 57376.0, 57344.0, 1.0], device="cuda")
+    x[1, :2] = torch.tensor([57344.0, -57344.0], device="cuda")      # the largest that scale 128 holds
+    x[2, 0], x[2, 1] = float("inf"), 65504.0
+    x[3, 0] = -float("inf")
+    x[4] = 65504.0
+    x[5, 3] = 2.0 ** -14
+    kv = Cache(mc, _gen(1), 1, 16, 1, hd, True)
+    slot, cu, table = _u32(range(6)), _u32([0, 6]), _u32([0])
+    k, v = torch.empty_like(x), torch.empty_like(x)
+    on.kv_write(kv.c, x.data_ptr(), x.data_ptr(), slot.data_ptr(), 6)
+    on.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), 1, 6, 1)
+    on.flush()
+    assert torch.equal(k, v)
+    assert torch.equal(torch.isinf(k), torch.isinf(x)) and torch.equal(k[torch.isinf(x)], x[torch.isinf(x)])
+    code, scale = R.e4m3(x)
+    want = (code.double() * scale.double()[..., None])
+    want = torch.where(want.abs() == 65536, want.sign() * 65504, want)[~torch.isinf(x)]
+    assert torch.equal(k[~torch.isinf(x)].double(), want)
+    assert k[0, 0] == 65504 and k[0, 1] == -65504 and k[0, 2] == 65504 and k[0, 3] == 61440 and (k[4] == 65504).all()
+
+
+@pytest.mark.parametrize("scale", [256.0, 300.0, 2.0 ** 15, 146.2857])
+def test_read_of_products_beyond_the_type(on, mc, scale):
+    """Codes and scales of any origin: a product rounds to fp16, what lies beyond 65536 is infinite, up to there the largest value."""
+    kv = Cache(mc, _gen(2), 16, 16, 1, 64, True)
+    kv.k.view(torch.uint8).copy_(torch.arange(256, device="cuda", dtype=torch.uint8).repeat(64).view(16, 1, 16, 64))
+    kv.v.copy_(kv.k)
+    for t in kv.scales:
+        t[:] = scale
+    cu, table = _u32([0, 256]), _u32(range(16))
+    k, v = (torch.empty(256, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+    on.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), 1, 256, 16)
+    on.flush()
+    y = kv.k.view(256, 64).double() * float(np.float32(scale))
+    want = torch.where((y.abs() >= 65504) & (y.abs() <= 65536), y.sign() * 65504, y).float().half()   # y has 4 + 24 bits: float is one rounding early only for 146.2857
+    got = k.clone()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    ok = ~torch.isnan(want)
+    assert torch.equal(torch.isinf(got[ok]), torch.isinf(want[ok]))
+    fin = ok & ~torch.isinf(want)
+    assert ((got[fin].double() - want[fin].double()).abs() <= want[fin].double().abs() * 2.0 ** -10).all()   # one step: the early rounding may fall on a tie
+    assert torch.equal(torch.nan_to_num(k), torch.nan_to_num(v))
