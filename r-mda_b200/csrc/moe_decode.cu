@@ -454,7 +454,8 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                 keep[n][e] = m == top[n][e] ? 1.0f : exp2_fast(top[n][e] - m);
                 moves |= m != top[n][e];
                 top[n][e] = m;
-                shift[n][e] = m == -INFINITY ? 0.0f : m - WEIGHT_SHIFT;
+                // taken off before WEIGHT_SHIFT is added: m - WEIGHT_SHIFT would round, from 2^27 on to a weight beyond fp16
+                shift[n][e] = m == -INFINITY ? 0.0f : m;
                 sum[n][e] *= keep[n][e];
             }
         }
@@ -475,7 +476,7 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             for (uint32_t n = 0; n < NT; n += 1) {
 #pragma unroll
                 for (uint32_t half = 0; half < 2; half += 1) {
-                    const float w0 = exp2_fast(x[i][n][half * 2u] - shift[n][0]), w1 = exp2_fast(x[i][n][half * 2u + 1u] - shift[n][1]);
+                    const float w0 = exp2_fast(x[i][n][half * 2u] - shift[n][0] + WEIGHT_SHIFT), w1 = exp2_fast(x[i][n][half * 2u + 1u] - shift[n][1] + WEIGHT_SHIFT);
                     sum[n][0] += w0 * inv[i][half];
                     sum[n][1] += w1 * inv[i][half];
                     // weights round to fp16 for the product (11 bits, as many as the output has); their sum does not

@@ -129,3 +129,54 @@ def test_read_of_products_beyond_the_type(on, mc, scale):
     fin = ok & ~torch.isinf(want)
     assert ((got[fin].double() - want[fin].double()).abs() <= want[fin].double().abs() * 2.0 ** -10).all()   # one step: the early rounding may fall on a tie
     assert torch.equal(torch.nan_to_num(k), torch.nan_to_num(v))
+
+
+# ---- scores far beyond fp32's whole numbers -----------------------------------------------------------
+def _whole(g, most, *shape):
+    return torch.randint(-most, most + 1, shape, device="cuda", generator=g).half()
+
+
+def _check_sharp(got, q, k, v, offset, scale):
+    """Whole queries and keys: scores are exact, and two that differ, differ by the scale at least.  With 2^-scale far below every
+    rounding a row is the mean of the values at its largest score.  Weights of the largest are equal but for 2^-20 (the two ways
+    of taking 2^x) and round to fp16 for the product, their sum does not: 2^-11 of the mean of |v|; the output rounds by 2^-11."""
+    h, g = q.shape[1], k.shape[1]
+    seen = torch.arange(k.shape[0], device="cuda")[None] <= torch.arange(q.shape[0], device="cuda")[:, None] + offset
+    assert torch.isfinite(got).all()
+    for a in range(h):
+        b = a // (h // g)
+        x = (q[:, a].double() @ k[:, b].double().T).masked_fill(~seen, -float("inf"))
+        p = (x == x.amax(-1, keepdim=True)).double()
+        p = p / p.sum(-1, keepdim=True)
+        o = p @ v[:, b].double()
+        tol = 2.0 ** -11 * o.abs() + 2.0 ** -25 + (2.0 ** -11 + 2.0 ** -19) * (p @ v[:, b].double().abs())
+        assert ((got[:, a].double() - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads,scale", [(8, 64.0), (8, 4096.0), (20, 1e4), (2, 3000.0)])
+def test_decode_scores_beyond_whole_numbers(on, mc, e4m3, hd, heads, scale):
+    g, kv_heads, page, lengths = _gen(int(scale) + heads), 2, 16, [1, 700, 33, 5000, 128]
+    need = [-(-n // page) for n in lengths]
+    kv = Cache(mc, g, sum(need), page, kv_heads, hd, e4m3)
+    order, at = torch.arange(sum(need), device="cuda", dtype=torch.int32), 0
+    table = torch.zeros(len(need), max(need), device="cuda", dtype=torch.int32)
+    for i, m in enumerate(need):
+        table[i, :m] = order[at:at + m]
+        at += m
+    total = sum(need) * page
+    k = _whole(g, 16, total, kv_heads, hd) * (4 if e4m3 else 5)   # 16 and below are e4m3 values at any power of two
+    v = _f16(g, total, kv_heads, hd).clamp_(-3.5, 3.5)
+    v[..., 0] = 4.0   # one scale for all values: rows of equal scores keep equal weights
+    slot = torch.arange(total, device="cuda", dtype=torch.int32)
+    on.kv_write(kv.c, k.data_ptr(), v.data_ptr(), slot.data_ptr(), total)
+    q, length = _whole(g, 64, len(lengths), heads, hd), _u32(lengths)
+    out = torch.full_like(q, 7.0)
+    on.attn_decode(kv.c, q.data_ptr(), table.data_ptr(), length.data_ptr(), out.data_ptr(), len(lengths), heads, max(lengths), max(need), scale=scale)
+    on.flush()
+    at = 0
+    for i, n in enumerate(lengths):
+        _, vv = kv.rows(table[i, :need[i]].long(), n)
+        _check_sharp(out[i:i + 1], q[i:i + 1], k[at * page:at * page + n], vv, n - 1, scale)
+        at += need[i]
