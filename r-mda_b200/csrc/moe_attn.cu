@@ -34,6 +34,8 @@
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 
+#include <string.h>
+
 namespace {
 
 using namespace moe_tc;
@@ -43,6 +45,10 @@ constexpr uint32_t HALF_BYTES = 128 * 128;       // 128 rows of 64 columns, one 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float GROW = 6.0f;                     // log2 of how far weights may pass the reference before a rescale
 constexpr float SHIFT = 8.0f;                    // weights are at most 2^(GROW + SHIFT) = 2^14; fp16 then goes down to 2^-32 of the reference
+// A row whose largest logit passes about 2^FAR (in log2 units) is scaled as if its exponent were that: powers of two come off the scale.
+// The product of reference and scale is rounded before it is taken off, by 1 at most up to 2^(FAR + 2), so weights stay below
+// 2^(GROW + SHIFT + 1); unbounded, they pass fp16.  fp32 scores are good to 2^-24 of themselves, so logits of that size to half a unit.
+constexpr int32_t FAR = 23;
 // Of every POLY_OF pairs of exponentials POLY_SHARE go to the multiply-add pipe.
 constexpr uint32_t POLY_OF = 4, POLY_SHARE = 1;
 // Items with a masked block that may be between their V check and their epilogue.  Each has such a block in the ring until its products
@@ -85,6 +91,7 @@ struct AttnArgs {
     uint32_t rows_q, rows_k, kv_heads, group, tile_tokens;
     uint32_t kv_stride, o_stride;
     float scale;
+    uint32_t far_top, far_scale;   // bits of the reference's exponent from which the scale is cut; those of the scale, and far_top more
     uint32_t *status;
     uint64_t wait_ns;
 };
@@ -578,14 +585,12 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t s_at = tmem + t * 128u + lanes, o_at = tmem + 256u + t * HD + lanes;
         const float to_log2 = a.scale * LOG2E;
-        const uint64_t scale2 = two(to_log2, to_log2);
         uint32_t s_phase = 0, sum_phase = 1, turn_phase = t == 0 ? 1u : 0u;   // the first tile begins
         bool ok = true;
         while (ok && items.next(a, p, head)) {
             const Blocks b = blocks_of(p, a.tile_tokens);
             const uint32_t n = b.tile[t], both = min(b.tile[0], b.tile[1]);   // blocks that both tiles have
             if (n == 0) continue;
-            const int32_t vis = visible(p, t * a.tile_tokens + my_token);
             const int32_t tile_first = visible(p, t * a.tile_tokens);
             float top = -INFINITY, sum = 0.0f;   // top: the reference that weights are taken against, in score units
             for (uint32_t j = n; j-- > 0;) {
@@ -600,7 +605,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     // some rows do not see all of the block: what they do not see becomes -infinity where it lies, so that the code
                     // below, which every block runs, is short (straight through once a block, it is bound by its own fetching); done
                     // while the other tile has its turn
-                    const int32_t seen = vis - (int32_t)(j * BLOCK_KEYS);   // columns below it are visible
+                    const int32_t seen = tile_first + (int32_t)my_token - (int32_t)(j * BLOCK_KEYS);   // columns below it are visible
 #pragma unroll 1
                     for (int32_t i = 0; i < 4; i += 1) {
                         if (__all_sync(0xffffffffu, seen >= i * 32 + 32)) continue;
@@ -665,8 +670,9 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     }
                 }
                 // against -infinity everything is -infinity: weights 0; against infinity or NaN everything is NaN
-                const float base = top == -INFINITY ? 0.0f : SHIFT - top * to_log2 + (top - top);
-                const uint64_t base2 = two(base, base);
+                const float scale = __uint_as_float(a.far_scale - max(__float_as_uint(top) & 0x7f800000u, a.far_top));
+                const float base = top == -INFINITY ? 0.0f : SHIFT - top * scale + (top - top);
+                const uint64_t scale2 = two(scale, scale), base2 = two(base, base);
                 uint64_t part[2] = {0, 0};
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i += 1) {
@@ -866,6 +872,12 @@ extern "C" void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k1
     a.kv_stride = pc.kv_stride;
     a.o_stride = pc.o_stride;
     a.scale = pc.scale;
+    const float to_log2 = pc.scale * LOG2E;
+    uint32_t bits;
+    memcpy(&bits, &to_log2, sizeof(bits));
+    const int32_t far = 127 + FAR - ((int32_t)(bits >> 23) - 127);
+    a.far_top = (uint32_t)(far < 255 ? far : 255) << 23;   // 255: not even infinity's; else the scale keeps an exponent of 22 there
+    a.far_scale = bits + a.far_top;
     a.status = c->dev_status_dev;
     a.wait_ns = c->wait_ns;
     const uint64_t pairs = (uint64_t)pc.rows_q / (2u * a.tile_tokens) + pc.seqs;   // at most

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from . import attn_ref as R
-from .test_gpu_attn import NO_SLOT, Attn, AttnRows, AttnW, Cache, _f16, _gen, _refused, _starts, _u32, on  # noqa: F401
+from .test_gpu_attn import NO_SLOT, Attn, AttnRows, AttnW, Cache, _attn, _f16, _gen, _refused, _starts, _u32, on  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -180,3 +180,34 @@ def test_decode_scores_beyond_whole_numbers(on, mc, e4m3, hd, heads, scale):
         _, vv = kv.rows(table[i, :need[i]].long(), n)
         _check_sharp(out[i:i + 1], q[i:i + 1], k[at * page:at * page + n], vv, n - 1, scale)
         at += need[i]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [64.0, 1000.0, 4096.0, 1e4])
+def test_attn_scores_beyond_whole_numbers(on, hd, scale):
+    """Logits of 10^8 and more: no weight overflows, none that counts is lost, and the maximum of a row is found across its blocks."""
+    g, heads, kv_heads, lq, lk = _gen(int(scale)), 6, 2, [300, 5, 1], [700, 5, 384]
+    q, k, v = _whole(g, 64, sum(lq), heads, hd), _whole(g, 64, sum(lk), kv_heads, hd), _f16(g, sum(lk), kv_heads, hd)
+    q[200:230] = 0   # rows of equal scores beside them in the same tile
+    out = torch.full_like(q, 7.0)
+    cu_q, cu_k = _starts(lq), _starts(lk)
+    on.attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), len(lq), sum(lq), sum(lk), heads, kv_heads, hd, scale=scale)
+    on.flush()
+    a = b = 0
+    for m, n in zip(lq, lk):
+        rows = [i for i in range(a, a + m) if not 200 <= i < 230]
+        lo, hi = (0, 200) if a == 0 else (0, m)
+        _check_sharp(out[a + lo:a + hi], q[a + lo:a + hi], k[b:b + n], v[b:b + n], n - m + lo, scale)
+        if a == 0:
+            _check_sharp(out[230:300], q[230:300], k[:n], v[:n], n - m + 230, scale)
+            o, mass, size = R.attention(q[200:230].double(), k[:n].double(), v[:n].double(), scale, n - m + 200)
+            R.check(out[200:230], o, mass, size, hd, n)
+        assert rows
+        a, b = a + m, b + n
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [1e-30, 1e-38, 1e-42])
+def test_attn_scales_next_to_zero(on, hd, scale):
+    """All visible keys weigh the same, masked ones nothing, down to scales below the normal numbers."""
+    _attn(on, _gen(7), [200, 3, 130], [200, 300, 130], 4, 2, hd, scale=scale)
