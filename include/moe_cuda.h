@@ -249,7 +249,9 @@ typedef struct moe_cuda_kv_t {
  * kept as 65536 and read back as 65504.  A NaN stays NaN and does not enter amax.
  * Infinities count as 65504 there, are kept as 448 * 256 and read back as
  * infinities; moe_cuda_attn_decode takes code * scale as it is, so there they
- * count as 114688 and the largest fp16 values as 65536.  Two rows with one slot: either may be kept, head by head. */
+ * count as 114688 and the largest fp16 values as 65536.
+ * A slot is in slot[] once: of two rows with one slot it would hold a mixture (one's
+ * codes with the other's scale), which is neither; no other slot is touched. */
 struct moe_pc_kv_write_t { uint32_t rows, stride; };
 void moe_cuda_kv_write(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const void *k16, const void *v16, const uint32_t *slot,
                        struct moe_pc_kv_write_t pc);

@@ -211,3 +211,26 @@ def test_attn_scores_beyond_whole_numbers(on, hd, scale):
 def test_attn_scales_next_to_zero(on, hd, scale):
     """All visible keys weigh the same, masked ones nothing, down to scales below the normal numbers."""
     _attn(on, _gen(7), [200, 3, 130], [200, 300, 130], 4, 2, hd, scale=scale)
+
+
+# ---- one slot, two rows ------------------------------------------------------------------------------
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_one_slot_twice_touches_no_other(on, mc, e4m3):
+    g = _gen(8)
+    kv = Cache(mc, g, 8, 16, 4, 128, e4m3)
+    rows = 100
+    x, y = _f16(g, rows, 512), _f16(g, rows, 512)
+    slot = torch.randperm(128, device="cuda", generator=g)[:rows].int()
+    slot[50:60] = slot[40]
+    slot[99] = slot[40]
+    before = [t.clone().view(torch.uint8) for t in (kv.k, kv.v)]
+    on.kv_write(kv.c, x.data_ptr(), y.data_ptr(), slot.data_ptr(), rows)
+    on.flush()
+    single = [i for i in range(rows) if int((slot == slot[i]).sum()) == 1]
+    for t, b, s in zip((kv.k, kv.v), before, (x, y)):
+        code = R.e4m3(s.view(rows, 4, 128))[0].view(torch.uint8) if e4m3 else s.view(rows, 4, 128).view(torch.uint8)
+        got = t.view(torch.uint8)
+        for i in single:
+            b[int(slot[i]) // 16, :, int(slot[i]) % 16] = code[i]
+        b[int(slot[40]) // 16, :, int(slot[40]) % 16] = got[int(slot[40]) // 16, :, int(slot[40]) % 16]
+        assert torch.equal(got, b)
