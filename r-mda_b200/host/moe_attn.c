@@ -81,14 +81,14 @@ static void moe_attn_end(moe_attn_t *q, const moe_attn_w_t *w, const moe_attn_ro
     moe_cuda_dense(q->c, q->o16, w->out, r->out, r->amax, pd);
 }
 
-void moe_attn_prompt(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t *w, const moe_attn_rows_t *r, const uint32_t *cu_q,
+bool moe_attn_prompt(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t *w, const moe_attn_rows_t *r, const uint32_t *cu_q,
                      const uint32_t *cu_k, uint32_t rows_k) {
-    if (r->rows == 0) return;
+    if (r->rows == 0) return moe_cuda_status(q->c) == MOE_OK;
     if (cu_k != NULL && rows_k > q->keys) {
         fprintf(stderr, "moe_attn: %u keys, room for %u\n", rows_k, q->keys);
-        return;
+        return false;
     }
-    if (!moe_attn_begin(q, kv, w, r)) return;
+    if (!moe_attn_begin(q, kv, w, r)) return false;
     struct moe_pc_attn_t pa = {
         .seqs = r->seqs,
         .rows_q = r->rows,
@@ -116,16 +116,17 @@ void moe_attn_prompt(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t 
         moe_cuda_attn(q->c, q->p16, q->k16, q->v16, cu_q, cu_k, q->o16, pa);
     }
     moe_attn_end(q, w, r);
+    return moe_cuda_status(q->c) == MOE_OK;
 }
 
-void moe_attn_step(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t *w, const moe_attn_rows_t *r, const uint32_t *len,
+bool moe_attn_step(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t *w, const moe_attn_rows_t *r, const uint32_t *len,
                    uint32_t max_len) {
-    if (r->rows == 0) return;
+    if (r->rows == 0) return moe_cuda_status(q->c) == MOE_OK;
     if (r->rows != r->seqs) {
         fprintf(stderr, "moe_attn: a step has one row per sequence\n");
-        return;
+        return false;
     }
-    if (!moe_attn_begin(q, kv, w, r)) return;
+    if (!moe_attn_begin(q, kv, w, r)) return false;
     struct moe_pc_attn_decode_t pa = {
         .seqs = r->seqs,
         .heads = q->heads,
@@ -137,4 +138,5 @@ void moe_attn_step(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t *w
     };
     moe_cuda_attn_decode(q->c, kv, q->p16, r->table, len, q->o16, pa);
     moe_attn_end(q, w, r);
+    return moe_cuda_status(q->c) == MOE_OK;
 }

@@ -234,3 +234,60 @@ def test_one_slot_twice_touches_no_other(on, mc, e4m3):
             b[int(slot[i]) // 16, :, int(slot[i]) % 16] = code[i]
         b[int(slot[40]) // 16, :, int(slot[40]) % 16] = got[int(slot[40]) // 16, :, int(slot[40]) % 16]
         assert torch.equal(got, b)
+
+
+# ---- the C host side ---------------------------------------------------------------------------------
+def _host(pkg, mc):
+    pkg.build.build_host()
+    L = C.CDLL(pkg.build.HOST_LIB)
+    L.moe_attn_open.restype = L.moe_attn_prompt.restype = L.moe_attn_step.restype = C.c_bool
+    L.moe_attn_open.argtypes = [C.POINTER(Attn), C.c_void_p] + [C.c_uint32] * 5 + [C.c_float, C.c_uint32, C.c_uint32]
+    L.moe_attn_close.argtypes = [C.POINTER(Attn)]
+    L.moe_attn_prompt.argtypes = [C.POINTER(Attn), C.POINTER(mc.Kv), C.POINTER(AttnW), C.POINTER(AttnRows), C.c_void_p, C.c_void_p, C.c_uint32]
+    L.moe_attn_step.argtypes = [C.POINTER(Attn), C.POINTER(mc.Kv), C.POINTER(AttnW), C.POINTER(AttnRows), C.c_void_p, C.c_uint32]
+    return L
+
+
+class _Layer:
+    """A layer's attention of 2 x 64 columns over 256, with a cache of one sequence."""
+
+    def __init__(self, on, pkg, mc, rot, rows, keys, seed=71):
+        self.L, self.d, self.h, self.g, self.hd, self.seed = _host(pkg, mc), 256, 2, 1, 64, seed
+        gen = _gen(seed)
+        self.q = Attn()
+        self.opened = self.L.moe_attn_open(C.byref(self.q), on.p, self.d, self.h, self.g, self.hd, rot, 1e4, rows, keys)
+        self.qkv, self.wo = _f16(gen, self.q.cols, self.d) * 0.06, _f16(gen, self.d, self.h * self.hd) * 0.05
+        self.w = AttnW(self.qkv.data_ptr(), self.wo.data_ptr())
+        self.kv = Cache(mc, gen, 16, 16, self.g, self.hd, False)
+        self.table = torch.arange(16, device="cuda", dtype=torch.int32)
+
+    def rows(self, rows, kept, seqs=1, value=7.0):
+        gen = _gen(self.seed + rows)
+        self.x, self.pos = _f16(gen, rows, self.d), torch.arange(rows, device="cuda", dtype=torch.int32)
+        self.slot = torch.where(self.pos < kept, self.pos, -1).int()
+        self.out = torch.full((rows, self.d), value, device="cuda")
+        return AttnRows(rows, seqs, self.x.data_ptr(), None, NO_SLOT, self.pos.data_ptr(), self.slot.data_ptr(), self.table.data_ptr(), 16, self.out.data_ptr())
+
+    def close(self):
+        self.L.moe_attn_close(C.byref(self.q))
+
+
+def test_host_attention_says_what_it_refuses(on, mc, pkg):
+    """Too many rows, too many keys, a step of other rows than sequences: false, nothing written, and the context goes on."""
+    y = _Layer(on, pkg, mc, 64, 8, 8)
+    assert y.opened
+    cu, length = _u32([0, 8]), _u32([8])
+    for run in (lambda r: y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), cu.data_ptr(), None, 0),
+                lambda r: y.L.moe_attn_step(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), length.data_ptr(), 16)):
+        assert run(y.rows(9, 9, 9)) is False and (y.out == 7).all()
+    r = y.rows(8, 8)
+    assert y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), cu.data_ptr(), cu.data_ptr(), 9) is False
+    assert y.L.moe_attn_step(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), length.data_ptr(), 16) is False
+    on.flush()
+    assert (y.out == 7).all()
+    assert y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), cu.data_ptr(), None, 0) is True
+    on.flush()
+    assert not (y.out == 7).any()
+    r0 = y.rows(0, 0)
+    assert y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r0), cu.data_ptr(), None, 0) is True   # nothing to do
+    y.close()
