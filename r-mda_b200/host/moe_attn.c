@@ -55,7 +55,7 @@ static bool moe_attn_begin(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_att
     struct moe_pc_rope_t pr = {
         .rows = r->rows,
         .heads = q->heads + 2u * q->kv_heads,
-        .rot_heads = q->heads + q->kv_heads,
+        .rot_heads = q->rot != 0 ? q->heads + q->kv_heads : 0,
         .hd = q->hd,
         .rot = q->rot,
         .stride = q->cols,

@@ -31,7 +31,7 @@ typedef struct moe_attn_w_t {
 
 /* (heads + 2 kv_heads) * hd rounded up to 128 */
 uint32_t moe_attn_cols(uint32_t heads, uint32_t kv_heads, uint32_t hd);
-/* keys: 0 if no prompt call will have cached prefixes.  d % 128 == 0. */
+/* rot: columns of a head that turn, 0 for none.  keys: 0 if no prompt call will have cached prefixes.  d % 128 == 0. */
 bool moe_attn_open(moe_attn_t *q, moe_cuda_ctx_t *c, uint32_t d, uint32_t heads, uint32_t kv_heads, uint32_t hd, uint32_t rot, float theta,
                    uint32_t rows, uint32_t keys);
 void moe_attn_close(moe_attn_t *q);

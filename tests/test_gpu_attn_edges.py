@@ -291,3 +291,18 @@ def test_host_attention_says_what_it_refuses(on, mc, pkg):
     r0 = y.rows(0, 0)
     assert y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r0), cu.data_ptr(), None, 0) is True   # nothing to do
     y.close()
+
+
+def test_host_attention_without_rotation(on, mc, pkg):
+    """rot 0: queries and keys stay as projected."""
+    y = _Layer(on, pkg, mc, 0, 8, 0)
+    cu = _u32([0, 8])
+    r = y.rows(8, 8)
+    y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), cu.data_ptr(), None, 0)
+    on.flush()
+    p = (y.x.double() @ y.qkv.double().T)[:, :4 * 64].view(8, 4, 64)
+    o, mass, size = R.attention(p[:, :2], p[:, 2:3], p[:, 3:], 0.125, 0)
+    # half a step of fp16 in queries, keys and values and in the weights of the second product; sums of 256 fp32 products
+    e = R.bound(o, mass, size, 64, 8) + mass * (2 * 2.0 ** -10 * size[..., None] * 1.1 + 2.0 ** -10)
+    assert ((y.out.double() - o.view(8, -1) @ y.wo.double().T).abs() <= e.view(8, -1) @ y.wo.double().abs().T * 1.01 + 1e-5).all()
+    y.close()
