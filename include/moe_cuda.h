@@ -276,6 +276,11 @@ struct moe_pc_attn_t { uint32_t seqs, rows_q, rows_k, heads, kv_heads, hd, q_str
 void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k16, const void *v16, const uint32_t *cu_q, const uint32_t *cu_k,
                    void *o16, struct moe_pc_attn_t pc);
 
+/* Rows *first .. rows-1 of out (row_bytes each, without gaps) become zero: what
+ * moe_cuda_attn leaves of a batch that is padded to `rows`, *first being the
+ * device's cu_q[seqs].  row_bytes % 16 == 0, out at a 16-byte address. */
+void moe_cuda_clear_behind(moe_cuda_ctx_t *c, void *out, const uint32_t *first, uint32_t rows, uint32_t row_bytes);
+
 /* Attention of one new token per sequence over the cache: query row s sees places
  * 0 .. len[s]-1 of sequence s (its own key and value have been written before).
  * len[s] == 0 gives 0.  max_len bounds len[] (a longer one is refused on the

@@ -72,6 +72,12 @@ static inline const char *moe_kv_read_refusal(const moe_cuda_kv_t *kv, const voi
     return NULL;
 }
 
+static inline const char *moe_clear_refusal(const void *out, const void *first, uint32_t rows, uint32_t row_bytes) {
+    if (row_bytes % 16u != 0) return "clear_behind: rows of a multiple of 16 bytes";
+    if (rows != 0 && row_bytes != 0 && (!moe_at16(out) || !moe_at4(first))) return "clear_behind: out at a 16-byte address, first";
+    return NULL;
+}
+
 static inline const char *moe_heads_refusal(uint32_t heads, uint32_t kv_heads) {
     if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0 || heads / kv_heads > MOE_ATTN_MAX_GROUP || kv_heads > 1024u)
         return "attention: 1 to 16 query heads for each of up to 1024 kv heads";

@@ -309,6 +309,13 @@ __global__ void __launch_bounds__(KV_THREADS, 6) moe_kv_read_kernel(const uint32
     }
 }
 
+// Almost always nothing to do: a block looks at *first and ends.
+__global__ void __launch_bounds__(KV_THREADS) moe_clear_behind_kernel(uint4 *out, const uint32_t *first, uint32_t rows, uint32_t row16) {
+    moe_pdl_begin();
+    const uint64_t end = (uint64_t)rows * row16, step = (uint64_t)gridDim.x * KV_THREADS;
+    for (uint64_t i = (uint64_t)*first * row16 + blockIdx.x * KV_THREADS + threadIdx.x; i < end; i += step) out[i] = make_uint4(0, 0, 0, 0);
+}
+
 KvArgs kv_args(moe_cuda_ctx *c, const moe_cuda_kv_t *kv) {
     KvArgs a;
     a.k = (uint8_t *)kv->k;
@@ -393,5 +400,15 @@ extern "C" void moe_cuda_kv_read(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, con
         if (kv->hd == 128u) moe_run(c, moe_kv_read_kernel<false, 16>, grid, KV_THREADS, 0, table, cu, k, v, a, pc, tile);
         else moe_run(c, moe_kv_read_kernel<false, 8>, grid, KV_THREADS, 0, table, cu, k, v, a, pc, tile);
     }
+    MOE_LAUNCHED(c);
+}
+
+extern "C" void moe_cuda_clear_behind(moe_cuda_ctx_t *c, void *out, const uint32_t *first, uint32_t rows, uint32_t row_bytes) {
+    if (!MOE_LIVE(c)) return;
+    const char *why = moe_clear_refusal(out, first, rows, row_bytes);
+    MOE_REQUIRE(c, why == NULL, "%s", why);
+    if (rows == 0 || row_bytes == 0) return;
+    moe_on_device on(c);
+    moe_run(c, moe_clear_behind_kernel, (uint32_t)c->sm_count, KV_THREADS, 0, (uint4 *)out, first, rows, row_bytes / 16u);
     MOE_LAUNCHED(c);
 }

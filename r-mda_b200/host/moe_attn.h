@@ -52,8 +52,9 @@ typedef struct moe_attn_rows_t {
 
 /* Both return false, with nothing enqueued, if the call does not fit (more rows than q->rows or keys than q->keys, a step whose rows
  * are not its sequences), and if the context has failed by then; what a kernel refuses shows at the next flush. */
-/* Prompts: sequence s has rows cu_q[s] .. cu_q[s+1]-1.  cu_k NULL: the sequences begin with them; else every sequence has
- * cu_k[s+1] - cu_k[s] keys in the cache by then, these rows' own among them, rows_k in all (at most q->keys). */
+/* Prompts: sequence s has rows cu_q[s] .. cu_q[s+1]-1, from 0 on; the output of rows behind the last one (a padded batch) is 0.
+ * cu_k NULL: the sequences begin with them; else every sequence has cu_k[s+1] - cu_k[s] keys in the cache by then, these rows' own
+ * among them, rows_k in all (at most q->keys). */
 bool moe_attn_prompt(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t *w, const moe_attn_rows_t *r, const uint32_t *cu_q,
                      const uint32_t *cu_k, uint32_t rows_k);
 /* One new token per sequence (rows == seqs); len[s] tokens with it, max_len at most. */

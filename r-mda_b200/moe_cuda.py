@@ -169,6 +169,7 @@ def lib() -> C.CDLL:
         L.moe_cuda_kv_write.argtypes = [vp, C.POINTER(Kv), vp, vp, vp, PcKvWrite]
         L.moe_cuda_kv_read.argtypes = [vp, C.POINTER(Kv), vp, vp, vp, vp, PcKvRead]
         L.moe_cuda_attn.argtypes = [vp, vp, vp, vp, vp, vp, vp, PcAttn]
+        L.moe_cuda_clear_behind.argtypes = [vp, vp, vp, u32, u32]
         L.moe_cuda_attn_decode.argtypes = [vp, C.POINTER(Kv), vp, vp, vp, vp, PcAttnDecode]
         L.moe_cuda_moe_rows.restype = u32
         L.moe_cuda_moe_rows.argtypes = [u32, u32, u32]
@@ -359,6 +360,9 @@ class Ctx:
                     kv_heads * hd if kv_stride is None else kv_stride, heads * hd if o_stride is None else o_stride,
                     hd ** -0.5 if scale is None else scale)
         lib().moe_cuda_attn(self.p, _ptr(q16), _ptr(k16), _ptr(v16), _ptr(cu_q), _ptr(cu_k), _ptr(o16), pc)
+
+    def clear_behind(self, out, first, rows, row_bytes):
+        lib().moe_cuda_clear_behind(self.p, _ptr(out), _ptr(first), rows, row_bytes)
 
     def attn_decode(self, kv, q16, table, length, o16, seqs, heads, max_len, table_stride, q_stride=None, o_stride=None, scale=None):
         n = heads * kv.hd

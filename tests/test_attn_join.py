@@ -55,3 +55,16 @@ def test_the_join_asks(parts):
     assert "n = moe_join_parts(first, split.w, gridDim.x / a.group)" in join and join.count("split.w") == 1
     assert re.search(r"if \(left != 0\) \{\s*gave_up = true;", text) and text.count("over = make_uint4(key.x") == 1
     assert "if (here && !ends && !gave_up && threadIdx.x == 0) over = make_uint4(key.x" in text
+
+
+@pytest.mark.parametrize("out,first,rows,row,ok", [(16, 4, 5, 32, True), (16, 4, 5, 24, False), (8, 4, 5, 32, False), (None, 4, 5, 32, False), (16, None, 5, 32, False),
+                                                    (16, 2, 5, 32, False), (None, None, 0, 32, True), (None, None, 5, 0, True)])
+def test_clear_refusals(tmp_path, out, first, rows, row, ok):
+    (tmp_path / "c.c").write_text('#include "%s/moe_attn_args.h"\n' % CSRC
+                                  + "const char *f(const void *o, const void *a, unsigned r, unsigned b) { return moe_clear_refusal(o, a, r, b); }\n")
+    so = tmp_path / "c.so"
+    r = subprocess.run(["gcc", "-std=gnu17", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC", "-o", str(so), str(tmp_path / "c.c")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    f = C.CDLL(str(so)).f
+    f.restype, f.argtypes = C.c_char_p, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32]
+    assert (f(out, first, rows, row) is None) == ok

@@ -306,3 +306,28 @@ def test_host_attention_without_rotation(on, mc, pkg):
     e = R.bound(o, mass, size, 64, 8) + mass * (2 * 2.0 ** -10 * size[..., None] * 1.1 + 2.0 ** -10)
     assert ((y.out.double() - o.view(8, -1) @ y.wo.double().T).abs() <= e.view(8, -1) @ y.wo.double().abs().T * 1.01 + 1e-5).all()
     y.close()
+
+
+def test_host_attention_of_a_padded_batch(on, mc, pkg):
+    """Rows behind the last sequence: their output is zero, whatever an earlier call has left in the buffers."""
+    y = _Layer(on, pkg, mc, 64, 40, 0)
+    whole, cu = _u32([0, 40]), _u32([0, 27])
+    r = y.rows(40, 40)
+    y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), whole.data_ptr(), None, 0)
+    on.flush()
+    full = y.out.clone()
+    r = y.rows(40, 27)
+    y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), cu.data_ptr(), None, 0)
+    on.flush()
+    assert torch.equal(y.out[:27], full[:27])   # causal: the same rows
+    assert (y.out[27:] == 0).all()
+    y.close()
+
+
+@pytest.mark.parametrize("rows,row,first", [(1, 16, 0), (40, 4096, 27), (40, 4096, 40), (40, 48, 41), (40, 48, 0xFFFFFFFF), (3000, 2048, 1)])
+def test_clear_behind(on, rows, row, first):
+    """Rows from *first on, none where that passes the rows, nothing behind them."""
+    out, at = torch.full((rows + 1, row), 7, device="cuda", dtype=torch.uint8), _u32([first])
+    on.clear_behind(out.data_ptr(), at.data_ptr(), rows, row)
+    on.flush()
+    assert (out[:min(first, rows)] == 7).all() and (out[min(first, rows):rows] == 0).all() and (out[rows] == 7).all()
