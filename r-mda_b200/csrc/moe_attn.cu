@@ -72,7 +72,8 @@ struct __align__(8) AttnBars {
     uint64_t sum_full[2], sum_empty[2];
     uint64_t turn[2];        // the tile's softmax may begin: the other one's has ended
     uint64_t drain[2];       // unwinding: all products issued have retired
-    uint32_t tmem_base, abort;
+    uint32_t tmem_base;
+    uint32_t abort[3];       // a role gave up; places of the ring that each tile has been through
     uint32_t found[FLAGS];   // the item's masked V blocks held something that is not finite
     float sum[2][TILE_ROWS];
 };
@@ -302,16 +303,19 @@ __device__ __forceinline__ void store32(__half *to, const uint32_t (&w)[8], bool
 // mbar_wait in two parts: the first looks stand where the wait is (a call would hold a softmax thread's registers to a calling
 // convention), all that bounds it is out of line.  Each role's step from item to item runs code that the others' have pushed
 // out of the instruction cache, so the code is kept short: 32 windows of 384 take 43.5 us, with the whole wait in every place 47.3.
+// Some waits last an item, however many keys it has, so the limit is for the time in which neither tile has moved: abort[1] and [2].
 __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t site, uint64_t wait_ns) {
-    uint32_t spins = 0;
+    uint32_t spins = 0, moved = 0;
     uint64_t t0 = 0;
     while (!mbar_try_wait(bar, parity)) {
         spins += 1;
         if ((spins & 0xffu) != 0) continue;
         if (*abort != 0) return false;
         const uint64_t now = globaltimer_ns();
-        if (t0 == 0) {
+        const uint32_t at = abort[1] + abort[2];
+        if (t0 == 0 || at != moved) {
             t0 = now;
+            moved = at;
         } else if (now - t0 > wait_ns) {
             *abort = 1;
             atomicCAS(status, 0u, (uint32_t)MOE_ERR_TIMEOUT | (site << 8));
@@ -340,7 +344,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     AttnBars<ST> *bars = reinterpret_cast<AttnBars<ST> *>(smem + C::SMEM);
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + 2u * C::TILE_BYTES;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    volatile uint32_t *abort = &bars->abort;
+    volatile uint32_t *abort = bars->abort;
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < ST; i += 1) {
@@ -361,7 +365,7 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             mbar_init(smem_u32(&bars->o_full[i]), 1);
             mbar_init(smem_u32(&bars->o_empty[i]), TILE_ROWS);
         }
-        bars->abort = 0;
+        bars->abort[0] = bars->abort[1] = bars->abort[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -513,7 +517,10 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     __syncwarp();
                     if (!ok) break;
                     if (j != 0) scores(ks, j - 1u < b.tile[t], j == 1u);
-                    if (elect_one()) umma_commit(smem_u32(&bars->kv_empty[vs]));
+                    if (elect_one()) {
+                        umma_commit(smem_u32(&bars->kv_empty[vs]));
+                        abort[1u + t] = at;
+                    }
                     __syncwarp();
                 }
             }

@@ -331,3 +331,17 @@ def test_clear_behind(on, rows, row, first):
     on.clear_behind(out.data_ptr(), at.data_ptr(), rows, row)
     on.flush()
     assert (out[:min(first, rows)] == 7).all() and (out[min(first, rows):rows] == 0).all() and (out[rows] == 7).all()
+
+
+# ---- waits ----------------------------------------------------------------------------------------------
+def test_attn_longer_than_the_wait_limit(on, mc):
+    """The limit is for a pipeline that does not move: a tile over two million keys takes many times it and ends in order."""
+    mc.lib().moe_cuda_set_wait_ns(on.p, 1_000_000)
+    g, n, hd = _gen(9), 2_000_000, 64
+    q, k, v = _f16(g, 8, 1, hd), _f16(g, n, 1, hd), _f16(g, n, 1, hd)
+    out = torch.full_like(q, 7.0)
+    cu_q, cu_k = _u32([0, 8]), _u32([0, n])
+    on.attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), 1, 8, n, 1, 1, hd)
+    on.flush()
+    o, mass, size = R.attention(q.double(), k.double(), v.double(), hd ** -0.5, n - 8)
+    R.check(out, o, mass, size, hd, n)
