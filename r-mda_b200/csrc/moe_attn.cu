@@ -71,7 +71,7 @@ struct __align__(8) AttnBars {
     uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];   // p_full: of each tile, keys 0-63 and 64-127
     uint64_t sum_full[2], sum_empty[2];
     uint64_t turn[2];        // the tile's softmax may begin: the other one's has ended
-    uint64_t drain[2];       // unwinding: all products issued have retired
+    uint64_t drain[2];       // at the end: all products issued have retired, and what waits for them has been told
     uint32_t tmem_base;
     uint32_t abort[3];       // a role gave up; places of the ring that each tile has been through
     uint32_t found[FLAGS];   // the item's masked V blocks held something that is not finite
@@ -525,13 +525,12 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 }
             }
             __syncwarp();
-            if (*abort != 0) {
-                // unwinding: a bounded time for the products already issued
-                if (elect_one()) umma_commit(smem_u32(&bars->drain[t]));
-                __syncwarp();
-                for (uint32_t spin = 0; spin < (1u << 16); spin += 1) {
-                    if (mbar_try_wait(smem_u32(&bars->drain[t]), 0)) break;
-                }
+            // Arrivals at the ring's last barriers may be under way still, and products when unwinding: the shared memory and tensor
+            // memory are theirs until then.  A bounded time for them.
+            if (elect_one()) umma_commit(smem_u32(&bars->drain[t]));
+            __syncwarp();
+            for (uint32_t spin = 0; spin < (1u << 16); spin += 1) {
+                if (mbar_try_wait(smem_u32(&bars->drain[t]), 0)) break;
             }
             __syncwarp();
         } else if (warp == 2) {
