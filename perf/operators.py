@@ -269,18 +269,22 @@ PLAIN = {"rope": _rope, "write": _write, "read": _read, "attn": _attn, "decode":
 
 # ---- one pass: the library's calls -------------------------------------------------------------
 _held = {}
+CUDA_STREAM_LEGACY = 1   # cudaStreamLegacy
 
 
-def _library():
-    """A program's one context, on a stream of its own."""
-    if not _held:
+def _library(s):
+    """A program's context on the stream that its tensors are made and used on; a state keeps the one it began with."""
+    if "library" not in s:
         import __graft_entry__ as entry
 
-        mc = entry.load_package().moe_cuda
-        stream = torch.cuda.Stream()
-        _held.update(mc=mc, stream=stream, ctx=mc.Ctx(torch.cuda.current_device(), stream.cuda_stream))
-        _held["ctx"].check()
-    return _held["mc"], _held["ctx"]
+        device, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+        if (device, stream) not in _held:
+            mc = entry.load_package().moe_cuda
+            # the default stream by the handle that names it: without a stream the context would make one of its own
+            _held[device, stream] = mc, mc.Ctx(device, stream or CUDA_STREAM_LEGACY)
+            _held[device, stream][1].check()
+        s["library"] = _held[device, stream]
+    return s["library"]
 
 
 def _kv(mc, s):
@@ -291,7 +295,7 @@ def _kv(mc, s):
 
 
 def _call(s):
-    mc, ctx = _library()
+    mc, ctx = _library(s)
     case = s["case"]
     h, g, d = HEADS[case["heads"]]
     op = case["op"]
