@@ -26,7 +26,7 @@ namespace {
 using namespace moe_tc;
 
 constexpr float LOG2E = 1.4426950408889634f;
-// Weights are exp2(x - max + WEIGHT_SHIFT): 2^10 at most, so that fp16 holds weights down to 2^-34 of the largest.
+// Weights are taken against the running maximum less WEIGHT_SHIFT: 2^10 at most, so that fp16 holds weights down to 2^-34 of the largest.
 constexpr float WEIGHT_SHIFT = 10.0f;
 
 struct DecArgs {
@@ -438,23 +438,24 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             }
         }
 
-        // ---- softmax: running maximum of each head, weights, their sum ----
+        // ---- softmax: running reference (the maximum less WEIGHT_SHIFT) of each head, weights, their sum ----
         bool moves = false;
         float shift[NT][2], keep[NT][2];
 #pragma unroll
         for (uint32_t n = 0; n < NT; n += 1) {
 #pragma unroll
             for (uint32_t e = 0; e < 2; e += 1) {
-                float m = top[n][e];
+                float m = fmaxf(x[0][n][e], x[0][n][2u + e]);
 #pragma unroll
-                for (uint32_t i = 0; i < SG; i += 1) m = fmaxf(m, fmaxf(x[i][n][e], x[i][n][2u + e]));
+                for (uint32_t i = 1; i < SG; i += 1) m = fmaxf(m, fmaxf(x[i][n][e], x[i][n][2u + e]));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                // rounded up: to nearest, from 2^27 on, weights could pass fp16
+                m = fmaxf(top[n][e], __fadd_ru(m, -WEIGHT_SHIFT));
                 keep[n][e] = m == top[n][e] ? 1.0f : exp2_fast(top[n][e] - m);
                 moves |= m != top[n][e];
                 top[n][e] = m;
-                // taken off before WEIGHT_SHIFT is added: m - WEIGHT_SHIFT would round, from 2^27 on to a weight beyond fp16
                 shift[n][e] = m == -INFINITY ? 0.0f : m;
                 sum[n][e] *= keep[n][e];
             }
@@ -476,7 +477,7 @@ moe_attn_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             for (uint32_t n = 0; n < NT; n += 1) {
 #pragma unroll
                 for (uint32_t half = 0; half < 2; half += 1) {
-                    const float w0 = exp2_fast(x[i][n][half * 2u] - shift[n][0] + WEIGHT_SHIFT), w1 = exp2_fast(x[i][n][half * 2u + 1u] - shift[n][1] + WEIGHT_SHIFT);
+                    const float w0 = exp2_fast(x[i][n][half * 2u] - shift[n][0]), w1 = exp2_fast(x[i][n][half * 2u + 1u] - shift[n][1]);
                     sum[n][0] += w0 * inv[i][half];
                     sum[n][1] += w1 * inv[i][half];
                     // weights round to fp16 for the product (11 bits, as many as the output has); their sum does not
