@@ -345,3 +345,32 @@ def test_attn_longer_than_the_wait_limit(on, mc):
     on.flush()
     o, mass, size = R.attention(q.double(), k.double(), v.double(), hd ** -0.5, n - 8)
     R.check(out, o, mass, size, hd, n)
+
+
+# ---- offsets that pass 32 bits ---------------------------------------------------------------------------
+def test_rows_far_apart(on, mc):
+    """Columns of rows 2^23 elements apart: projection, positions, cache and prompt attention beyond 2^32 elements."""
+    g, rows, h, kv_heads, hd, stride = _gen(12), 600, 4, 2, 64, 2 ** 23 + 8
+    cols = (h + 2 * kv_heads) * hd
+    x = torch.empty(rows, stride, device="cuda")
+    x[:, :cols] = torch.randn(rows, cols, device="cuda", generator=g)
+    p = torch.empty(rows, stride, device="cuda", dtype=torch.float16)
+    p[:, cols:cols + 8] = 7.0
+    out = torch.empty(rows, stride, device="cuda", dtype=torch.float16)
+    out[:, h * hd:h * hd + 8] = 7.0
+    pos, cu = torch.zeros(rows, device="cuda", dtype=torch.int32), _u32([0, rows])
+    on.rope(x.data_ptr(), pos.data_ptr(), p.data_ptr(), rows, h + 2 * kv_heads, h + kv_heads, hd, hd, 1e4, stride, stride)
+    at = p.data_ptr()
+    on.attn(at, at + 2 * h * hd, at + 2 * (h + kv_heads) * hd, cu.data_ptr(), cu.data_ptr(), out.data_ptr(), 1, rows, rows, h, kv_heads, hd, stride, stride, stride)
+    kv = Cache(mc, g, -(-rows // 16), 16, kv_heads, hd, False)
+    slot = torch.arange(rows, device="cuda", dtype=torch.int32)
+    on.kv_write(kv.c, at + 2 * h * hd, at + 2 * (h + kv_heads) * hd, slot.data_ptr(), rows, stride)
+    table, back = torch.arange(-(-rows // 16), device="cuda", dtype=torch.int32), [out[:, 1024:], out[:, 2048:]]
+    on.kv_read(kv.c, table.data_ptr(), cu.data_ptr(), back[0].data_ptr(), back[1].data_ptr(), 1, rows, table.numel(), stride)
+    on.flush()
+    y = x[:, :cols].half()   # position 0 turns nothing
+    assert torch.equal(p[:, :cols], y) and (p[:, cols:cols + 8] == 7).all() and (out[:, h * hd:h * hd + 8] == 7).all()
+    q, k, v = (y[:, a * hd:b * hd].reshape(rows, -1, hd) for a, b in ((0, h), (h, h + kv_heads), (h + kv_heads, h + 2 * kv_heads)))
+    for t, w in zip(back, (k, v)):
+        assert torch.equal(t[:, :kv_heads * hd], w.reshape(rows, -1))
+    R.check(out[:, :h * hd].reshape(rows, h, hd), *R.attention(q.double(), k.double(), v.double(), hd ** -0.5, 0), hd, rows)
