@@ -209,7 +209,12 @@ void moe_cuda_dense(moe_cuda_ctx_t *c, const void *A16, const void *W, float *C,
  * host/moe_attn.c composes the calls.
  *
  * Operands are fp16 at 16-byte addresses, rows at strides that are multiples of
- * 8 elements; sums, softmax statistics and angles are fp32 or wider.  A group of
+ * 8 elements; sums, softmax statistics and angles are fp32 or wider.  Softmax
+ * weights round to fp16 for their product with the values (their sum does not),
+ * against a reference below which fp16 goes down to 2^-32 of the largest; their
+ * exponentials are good to 2^-18.  A visible key or value that is not finite
+ * makes what depends on it infinite or NaN; which of the two is not promised.
+ * A scale is positive, 10^4 at most.  A group of
  * heads / kv_heads query heads shares a key-value head: query head j reads head
  * j / (heads / kv_heads).  A call on a context whose device is not the current
  * one runs on the context's device.  None of them allocates, so all of them can
@@ -271,7 +276,11 @@ void moe_cuda_kv_read(moe_cuda_ctx_t *c, const moe_cuda_kv_t *kv, const uint32_t
  * sees keys 0 .. i + lk - lq.  o = softmax(scale * q k^T) v per head; a query that
  * sees nothing gives 0; keys and values that a query does not see do not matter to
  * it, whatever they hold.  Output rows behind cu_q[seqs] are left as they were.
- * hd 64 or 128; heads / kv_heads from 1 to 16; row counts below 2^31. */
+ * In a row whose largest logit passes 2^23 (about; in units of log 2) logits are
+ * scaled down by the powers of two above it, which fp32 scores cannot resolve.
+ * hd 64 or 128; heads / kv_heads from 1 to 16; row counts below 2^31.  Several
+ * sequences take 16 bytes of the work area for each, and for every 256 rows of
+ * query heads that share a key-value head (else MOE_ERR_NOMEM). */
 struct moe_pc_attn_t { uint32_t seqs, rows_q, rows_k, heads, kv_heads, hd, q_stride, kv_stride, o_stride; float scale; };
 void moe_cuda_attn(moe_cuda_ctx_t *c, const void *q16, const void *k16, const void *v16, const uint32_t *cu_q, const uint32_t *cu_k,
                    void *o16, struct moe_pc_attn_t pc);

@@ -4,7 +4,7 @@
  * attention, output projection.  What mda_qwen_attn_rec is to the reference's
  * layer (src/qwen.c, between the two mda_qwen_res_rec of mda_qwen_layer_rec),
  * for a plain causal softmax with grouped heads and a cache that the reference
- * does not keep.
+ * does not keep.  The calling thread's current device is the context's.
  */
 #ifndef MOE_ATTN_H
 #define MOE_ATTN_H
