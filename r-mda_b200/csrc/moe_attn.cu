@@ -722,27 +722,27 @@ moe_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const uint32_t row = (warp & 3u) * 32u + lane, my_token = row / a.group, my_head = row - my_token * a.group;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const bool whole = ((uintptr_t)a.o & 31u) == 0 && a.o_stride % 16u == 0;
-        uint32_t phase[2] = {0, 0}, n_item = 0;
+        uint32_t phase = 0, n_item = 0;   // phase: a bit for each tile
         bool ok = true;
         while (ok && items.next(a, p, head)) {
             const Blocks b = blocks_of(p, a.tile_tokens);
             const uint32_t flag = n_item % FLAGS;
             if (b.masks()) n_item += 1;
-#pragma unroll
+#pragma unroll 1
             for (uint32_t t = 0; t < 2; t += 1) {
                 const uint32_t token = t * a.tile_tokens + my_token;   // behind the pair's first
                 const bool mine = my_token < a.tile_tokens && token < p.left;
                 __half *out = a.o + (size_t)(p.q_row + token) * a.o_stride + (size_t)(head * a.group + my_head) * HD;
-                if (b.tile[t] == 0) {   // no query, or none that sees a key
+                if ((t == 0 ? b.tile[0] : b.tile[1]) == 0) {   // no query, or none that sees a key
                     if (mine) {
-#pragma unroll
+#pragma unroll 1
                         for (uint32_t i = 0; i < HD; i += 8) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
                     }
                     continue;
                 }
-                ok = ok && AT_WAIT(&bars->sum_full[t], phase[t], 43) && AT_WAIT(&bars->o_full[t], phase[t], 44);
+                ok = ok && AT_WAIT(&bars->sum_full[t], phase >> t & 1u, 43) && AT_WAIT(&bars->o_full[t], phase >> t & 1u, 44);
                 if (!ok) break;
-                phase[t] ^= 1u;
+                phase ^= 1u << t;
                 __syncwarp();
                 tc_fence_after();
                 const float sum = bars->sum[t][row];
