@@ -26,11 +26,12 @@
 // the rows that do see them get them added at the end from global memory (a weight is positive, so infinities keep their sign).
 // A NaN score makes the row's maximum NaN, and with it the whole row.
 //
-// One B200: a prompt of 4096 (32 heads of 128, 4 kv heads) 123 us = 1120 TFLOP/s, 0.68 of the measured bf16 rate; one of 8192
-// 460 us = 1195 in short bursts and 533 = 1030 back to back, under the power cap; 13 prompts up to 1999 behind 517 cached
-// tokens (12 heads of 64) 104 us; 32 windows of 384 (16 heads of 128, 2 kv heads) 43.5 us (both captured, with the plan kernel).  On long prompts the tensor pipe is busy
-// 0.57 and the exp2 unit 0.43 of the time: what is left is the softmax's own turn, ~1700 cycles a tile and block.  Short
-// prompts are bound by the steps between items (~3500 cycles) and by blocks cut by the diagonal.
+// One B200: a prompt of 8192 (32 heads of 128, 4 kv heads) 465 us = 1183 TFLOP/s, 0.71 of the measured bf16 rate, in bursts of a few
+// milliseconds, and 532 us = 1033 for seconds on end, at 1515 MHz of 1965 under the 1000 W cap; one of 4096 128 us = 1073 and 143 us =
+// 959 (1590 MHz); 13 prompts up to 1999 behind 517 cached tokens (12 heads of 64) 107 us, 103 captured; 32 windows of 384 (16 heads
+// of 128, 2 kv heads) 50 us back to back, 45 captured, with the plan kernel.  On long prompts the tensor pipe is busy 0.58 and the exp2
+// unit 0.44 of the time: what is left is the softmax's own turn, ~1700 cycles a tile and block, of which 768 are the exp2 unit's.  Short
+// prompts are bound by the steps between items (~3500 cycles), by blocks cut by the diagonal and by the deal of few items.
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 
@@ -302,7 +303,8 @@ __device__ __forceinline__ void store32(__half *to, const uint32_t (&w)[8], bool
 
 // mbar_wait in two parts: the first looks stand where the wait is (a call would hold a softmax thread's registers to a calling
 // convention), all that bounds it is out of line.  Each role's step from item to item runs code that the others' have pushed
-// out of the instruction cache, so the code is kept short: 32 windows of 384 take 43.5 us, with the whole wait in every place 47.3.
+// out of the instruction cache, so the code is kept short: with the whole wait in every place 32 windows of 384 took 47.3 us captured,
+// with this 43.5.
 // Some waits last an item, however many keys it has, so the limit is for the time in which neither tile has moved: abort[1] and [2].
 __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t site, uint64_t wait_ns) {
     uint32_t spins = 0, moved = 0;

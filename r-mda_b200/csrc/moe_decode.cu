@@ -15,9 +15,9 @@
 // registers (the order of K's columns inside a product is free, Q's is the same).  A group is 8 of the 64 rows that the
 // 5th-generation tensor cores' smallest product has, and the products are far from a bound here.
 //
-// One B200: 129 sequences of up to 8191 tokens, fp16, 4 kv heads of 128 (1.08 GB) 171 us, of which this kernel 166 = 6.5 TB/s, the
-// copy rate; 16 of up to 16384, e4m3 (141 MB) 36.6 us, bound by the chain from codes to products in 8 warps and ~7 us of join and gaps; one of
-// 777 tokens 9.5 us with the call, a chain of latencies: the line, the first loads, the joins.
+// One B200: 129 sequences of up to 8191 tokens, fp16, 4 kv heads of 128 (1.08 GB) 173 us, of which this kernel 166 = 6.5 TB/s, the
+// copy rate; 16 of up to 16384, e4m3 (141 MB) 37 us, bound by the chain from codes to products in 8 warps (0.37 of the issue slots) and
+// ~7 us of join and gaps; one of 777 tokens 9.3 us with the call, a chain of latencies: the line, the first loads, the joins.
 #include "moe_attn.cuh"
 #include "moe_tc.cuh"
 

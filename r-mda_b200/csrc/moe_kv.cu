@@ -3,8 +3,8 @@
 // Each reads its input once and writes its output once.  The floor is HBM's, but what bound the first forms of all three was
 // instruction issue: hence multiplications for divisions, fp16x2 arithmetic, and a thread that has keys and values of a head.
 // One B200, back to back: rope of 4096 rows of 40 heads of 128, half rotated, 25.6 us = 4.9 TB/s (0.75 of the copy rate); write of
-// 16384 rows of 16 heads of 128 as e4m3 36-38 us = 5.4-5.7 TB/s; read of 12 prefixes of up to 8191 tokens, e4m3, 31.4 us = 5.5 TB/s.
-// Steps of 16 to 1003 rows take 1.6 to 2.4 us.
+// 16384 rows of 16 heads of 128 as e4m3 38 us = 5.4 TB/s (34 captured); read of 12 prefixes of up to 8191 tokens, e4m3, 31.4 us = 5.5
+// TB/s.  Steps of 16 to 1003 rows take 1.6 to 2.5 us on the GPU.
 #include "moe_attn.cuh"
 
 namespace {
