@@ -116,7 +116,12 @@ bool moe_attn_prompt(moe_attn_t *q, const moe_cuda_kv_t *kv, const moe_attn_w_t 
         moe_cuda_attn(q->c, q->p16, q->k16, q->v16, cu_q, cu_k, q->o16, pa);
     }
     /* rows of a padded batch: nothing attends there, and an earlier call's output is not this one's */
-    moe_cuda_clear_behind(q->c, q->o16, cu_q + r->seqs, r->rows, q->heads * q->hd * (uint32_t)sizeof(uint16_t));
+    uint32_t row = q->heads * q->hd * (uint32_t)sizeof(uint16_t);
+    if (r->seqs != 0) {
+        moe_cuda_clear_behind(q->c, q->o16, cu_q + r->seqs, r->rows, row);
+    } else { /* no sequence, so perhaps no offsets */
+        moe_cuda_fill(q->c, q->o16, (uint64_t)r->rows * row, 0);
+    }
     moe_attn_end(q, w, r);
     return moe_cuda_status(q->c) == MOE_OK;
 }

@@ -324,6 +324,19 @@ def test_host_attention_of_a_padded_batch(on, mc, pkg):
     y.close()
 
 
+def test_host_attention_of_no_sequence(on, mc, pkg):
+    """Rows, but no sequence, and no offsets: all of the output is zero."""
+    y = _Layer(on, pkg, mc, 64, 40, 0)
+    r = y.rows(40, 40)
+    cu = _u32([0, 40])
+    assert y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), cu.data_ptr(), None, 0)
+    r = y.rows(40, 0, seqs=0)
+    assert y.L.moe_attn_prompt(C.byref(y.q), C.byref(y.kv.c), C.byref(y.w), C.byref(r), None, None, 0)
+    on.flush()
+    assert (y.out == 0).all()
+    y.close()
+
+
 @pytest.mark.parametrize("rows,row,first", [(1, 16, 0), (40, 4096, 27), (40, 4096, 40), (40, 48, 41), (40, 48, 0xFFFFFFFF), (3000, 2048, 1)])
 def test_clear_behind(on, rows, row, first):
     """Rows from *first on, none where that passes the rows, nothing behind them."""
